@@ -160,7 +160,8 @@ def _quantise(x, cache):
     x / scale to the nearest, ties to even, all in 32 bits. A row with an infinity or NaN has
     the scale NaN and codes 0."""
     x = x.float()
-    scale = (x.abs().amax(-1) / TOP[cache]).clamp(min=LEAST_SCALE)
+    # (a tensor divisor: torch multiplies by the reciprocal of a plain number)
+    scale = (x.abs().amax(-1) / torch.full((), TOP[cache], device=x.device)).clamp(min=LEAST_SCALE)
     scale = torch.where(scale.isfinite(), scale, torch.full_like(scale, math.nan))
     y = (x / scale[..., None]).clamp(-TOP[cache], TOP[cache]).nan_to_num(0.0)
     return (y.round() if cache == "int8" else y).to(CODES[cache]), scale
