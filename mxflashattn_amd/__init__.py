@@ -16,7 +16,14 @@ from .dispatch import (
     DispatchInfo,
     get_last_dispatch_info,
 )
-from .native import append_kv, paged_decode_split, reshape_and_cache
+from .native import (
+    append_kv,
+    gather_cache,
+    paged_decode_split,
+    paged_prefill,
+    quantize_and_cache,
+    reshape_and_cache,
+)
 from .policy import AdaptiveDispatchPolicy, DispatchDecision, DispatchPolicyConfig, WorkloadShape
 
 __all__ = [
@@ -31,8 +38,11 @@ __all__ = [
     "flash_attn_func",
     "flash_attn_varlen_func",
     "flash_attn_with_kvcache",
+    "gather_cache",
     "get_last_dispatch_info",
     "paged_decode_split",
+    "paged_prefill",
+    "quantize_and_cache",
     "reshape_and_cache",
     "summarize_error",
     "WorkloadShape",

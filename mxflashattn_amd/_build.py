@@ -25,7 +25,11 @@ LIB_PATH = LIB_DIR / LIB_NAME
 SOURCES = ("split_decode.hip", "split_hd64.hip", "split_hd64_ws.hip", "split_hd64_ws4.hip",
            "split_hd128.hip", "split_hd128_ws.hip", "split_hd128_ws4.hip", "split_hd256.hip",
            "split_hd256_ws.hip", "split_hd256_ws4.hip", "split_hd64_wide.hip",
-           "split_hd128_wide.hip", "kv_append.hip", "stream_read.hip")
+           "split_hd128_wide.hip", "split_hd64_rows_f16.hip", "split_hd64_rows_bf16.hip",
+           "split_hd128_rows_f16.hip",
+           "split_hd128_rows_bf16.hip", "split_hd256_rows_f16.hip", "split_hd256_rows_bf16.hip",
+           "prefill_hd64.hip", "prefill_hd128.hip", "prefill_hd256.hip",
+           "paged_prefill.hip", "kv_append.hip", "kv_quant.hip", "stream_read.hip")
 # Comparison build: QK always on the matrix cores (the default build puts it on
 # the VALU for launches of few columns at head dims >= 128).
 QK_MFMA_LIB_PATH = PACKAGE_DIR / "_lib" / "qk_mfma" / "libmxfa_mi355x.so"
@@ -100,7 +104,10 @@ _REMARK = re.compile(r"remark:\s+(Function Name|VGPRs Spill|ScratchSize \[bytes/
 # array indexed at run time) in another memory: it fails the build too.
 # Dynamic LDS (the tile prefix sums, the per-sequence kernel's pieces) is not
 # counted in the remark.
-STATIC_LDS_LIMITS = {"split_combine_kernel": 256 * 6 * 4}
+# (The prefill's tiles: two buffers of K and of V, 64 rows of up to 512 bytes, their
+# scales, and its work search.)
+STATIC_LDS_LIMITS = {"split_combine_kernel": 256 * 6 * 4,
+                     "paged_prefill_kernel": 4 * 64 * 512 + 2048}
 STATIC_LDS_DEFAULT = 64
 
 

@@ -83,6 +83,83 @@ int mxfa_package_contiguous_decode_launch(
     int q_heads, int kv_heads, int head_dim, int page_size, int dtype, int num_splits,
     void *stream);
 
+// Element type of an int8 cache (codes with one scale for each token and kv head), beside
+// the MXFA_DTYPE_* values of the C ABI.
+#define MXFA_PACKAGE_DTYPE_INT8 3
+
+// mxfa_split_decode_multi_launch (same arguments, checks and results, at most 16 columns)
+// over an 8-bit cache with one scale for each token and kv head: kv_dtype
+// MXFA_DTYPE_FP8_E4M3 or MXFA_PACKAGE_DTYPE_INT8, k_scales and v_scales fp32
+// [num_pages][HKV][PS] (strides of page and head in elements, tokens consecutive). A row's
+// scale that is not finite makes every query that sees the row NaN. num_splits from
+// mxfa_package_num_splits with fp8 != 0 and 16 columns.
+int mxfa_package_decode_rows_launch(
+    const void *q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h, int q_len,
+    int causal, int window_left, const float *sinks, float softcap, const float *alibi_slopes,
+    const void *k_cache, const void *v_cache, int64_t cache_stride_page,
+    int64_t cache_stride_token, int64_t cache_stride_head, const float *k_scales,
+    int64_t ks_stride_page, int64_t ks_stride_head, const float *v_scales, int64_t vs_stride_page,
+    int64_t vs_stride_head, const int32_t *block_table, int64_t bt_stride, const int32_t *seqlens,
+    int seqlen_add, void *out, int64_t out_stride_b, int64_t out_stride_t, int64_t out_stride_h,
+    void *workspace, size_t workspace_bytes, float scale, int batch, int q_heads, int kv_heads,
+    int head_dim, int page_size, int block_table_width, int num_pages, int dtype, int kv_dtype,
+    int num_splits, void *stream);
+
+// Attention of a chunk of new tokens over a paged cache (prefill_kernels.h). Query rows
+// [cu_seqlens_q[b], cu_seqlens_q[b + 1]) of q [rows_q, HQ, HD] are the last tokens of
+// sequence b, whose seqlens[b] keys (those of the chunk among them) lie in the pages of
+// block_table's row b: the n tokens sit at positions seqlens[b] - n on. causal, window_left,
+// softcap, sinks and alibi_slopes as mxfa_split_decode_multi_launch; a row that sees no key
+// gets zeros, and rows of no sequence are left as they were. Caches of `dtype`
+// (cache_dtype == dtype) or of 8 bits: MXFA_DTYPE_FP8_E4M3 or MXFA_PACKAGE_DTYPE_INT8 with
+// k_scales/v_scales (fp32, [num_pages][HKV][PS], strides of page and head in elements, tokens
+// consecutive) and/or k_scale/v_scale (one fp32 each; null: 1). Strides in elements, caches'
+// multiples of 16 bytes, q's of 8 elements, out's of 4. Offsets, lengths and page ids are held
+// to what exists, so wrong ones give wrong numbers, never an access out of range.
+// Two launches on `stream` where row tiles may be cut (a workspace of
+// mxfa_package_prefill_workspace_size bytes, contents of no matter), else one. Calls that
+// share a workspace must not overlap in time.
+int mxfa_package_prefill_workspace_size(int batch, int rows_q, int q_heads, int kv_heads,
+                                        int head_dim, int page_size, int block_table_width,
+                                        int num_cus, size_t *bytes);
+int mxfa_package_prefill_launch(
+    const void *q, int64_t q_stride_t, int64_t q_stride_h, int rows_q,
+    const int32_t *cu_seqlens_q, const void *k_cache, const void *v_cache,
+    int64_t cache_stride_page, int64_t cache_stride_token, int64_t cache_stride_head,
+    const float *k_scales, int64_t ks_stride_page, int64_t ks_stride_head, const float *v_scales,
+    int64_t vs_stride_page, int64_t vs_stride_head, const float *k_scale, const float *v_scale,
+    const int32_t *block_table, int64_t bt_stride, const int32_t *seqlens, void *out,
+    int64_t out_stride_t, int64_t out_stride_h, void *workspace, size_t workspace_bytes,
+    float scale, int causal, int window_left, float softcap, const float *sinks,
+    const float *alibi_slopes, int batch, int q_heads, int kv_heads, int head_dim, int page_size,
+    int block_table_width, int num_pages, int dtype, int cache_dtype, int num_cus, void *stream);
+
+// Rows of K and V ([num_tokens, HKV, HD], strides of token and head) quantised into 8-bit
+// caches at their slots, one scale for each token and head (kv_quant.hip); slots below 0 or
+// past the cache are skipped. Cache strides in bytes (multiples of 16), scales as above. Of
+// two tokens with one slot either may end up there, its codes and scale not always together.
+int mxfa_package_quantize_and_cache_launch(
+    const void *key, const void *value, int64_t kv_stride_token, int64_t kv_stride_head,
+    void *k_cache, void *v_cache, int64_t cache_stride_page, int64_t cache_stride_token,
+    int64_t cache_stride_head, float *k_scales, int64_t ks_stride_page, int64_t ks_stride_head,
+    float *v_scales, int64_t vs_stride_page, int64_t vs_stride_head, const int64_t *slot_mapping,
+    int num_tokens, int kv_heads, int head_dim, int page_size, int num_pages, int dtype,
+    int cache_dtype, void *stream);
+
+// The first cu_seqlens[b + 1] - cu_seqlens[b] tokens of every sequence, from their pages to
+// rows [cu_seqlens[b], cu_seqlens[b + 1]) of k_out and v_out ([total, HKV, HD] of `dtype`,
+// strides of token and head in elements, multiples of 8). Rows of no sequence, and those
+// past the block table's row, are left as they were.
+int mxfa_package_gather_cache_launch(
+    const void *k_cache, const void *v_cache, int64_t cache_stride_page,
+    int64_t cache_stride_token, int64_t cache_stride_head, const float *k_scales,
+    int64_t ks_stride_page, int64_t ks_stride_head, const float *v_scales, int64_t vs_stride_page,
+    int64_t vs_stride_head, const float *k_scale, const float *v_scale,
+    const int32_t *block_table, int64_t bt_stride, const int32_t *cu_seqlens, void *k_out,
+    void *v_out, int64_t out_stride_token, int64_t out_stride_head, int batch,
+    int block_table_width, int total, int kv_heads, int head_dim, int page_size, int num_pages,
+    int dtype, int cache_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

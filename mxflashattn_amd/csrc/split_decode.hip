@@ -76,6 +76,43 @@ int launch_probe_64(const DecodeParams &p, const Grid &g, int nbuf, uint32_t *si
 int launch_probe_128(const DecodeParams &p, const Grid &g, int nbuf, uint32_t *sink,
                      hipStream_t st);
 
+int launch_rows_64_f16(const DecodeParams &p, const Grid &g, int kind, bool wave_scan,
+                       hipStream_t st);
+int launch_seq_rows_64_f16(const DecodeParams &p, int kind, hipStream_t st);
+int launch_rows_64_bf16(const DecodeParams &p, const Grid &g, int kind, bool wave_scan,
+                       hipStream_t st);
+int launch_seq_rows_64_bf16(const DecodeParams &p, int kind, hipStream_t st);
+int launch_rows_128_f16(const DecodeParams &p, const Grid &g, int kind, bool wave_scan,
+                       hipStream_t st);
+int launch_seq_rows_128_f16(const DecodeParams &p, int kind, hipStream_t st);
+int launch_rows_128_bf16(const DecodeParams &p, const Grid &g, int kind, bool wave_scan,
+                       hipStream_t st);
+int launch_seq_rows_128_bf16(const DecodeParams &p, int kind, hipStream_t st);
+int launch_rows_256_f16(const DecodeParams &p, const Grid &g, int kind, bool wave_scan,
+                       hipStream_t st);
+int launch_seq_rows_256_f16(const DecodeParams &p, int kind, hipStream_t st);
+int launch_rows_256_bf16(const DecodeParams &p, const Grid &g, int kind, bool wave_scan,
+                       hipStream_t st);
+int launch_seq_rows_256_bf16(const DecodeParams &p, int kind, hipStream_t st);
+
+// The decode kernels over 8-bit rows with a scale each.
+static int launch_rows(const DecodeParams &p, const Grid &g, int hd, int dtype, int kind,
+                       bool wave_scan, hipStream_t st) {
+  const bool bf16 = dtype == MXFA_DTYPE_BF16;
+  const auto kernel = hd == 64    ? (bf16 ? launch_rows_64_bf16 : launch_rows_64_f16)
+                      : hd == 128 ? (bf16 ? launch_rows_128_bf16 : launch_rows_128_f16)
+                                  : (bf16 ? launch_rows_256_bf16 : launch_rows_256_f16);
+  return kernel(p, g, kind, wave_scan, st);
+}
+
+static int launch_seq_rows(const DecodeParams &p, int hd, int dtype, int kind, hipStream_t st) {
+  const bool bf16 = dtype == MXFA_DTYPE_BF16;
+  const auto kernel = hd == 64    ? (bf16 ? launch_seq_rows_64_bf16 : launch_seq_rows_64_f16)
+                      : hd == 128 ? (bf16 ? launch_seq_rows_128_bf16 : launch_seq_rows_128_f16)
+                                  : (bf16 ? launch_seq_rows_256_bf16 : launch_seq_rows_256_f16);
+  return kernel(p, kind, st);
+}
+
 static bool aligned16(const void *ptr) { return ((uintptr_t)ptr & 15u) == 0; }
 
 static int ilog2_exact(int v) {
@@ -128,7 +165,10 @@ struct SplitArgs {
   size_t ws_bytes;
   float scale;
   int batch, hq, hkv, hd, ps, btw, num_pages, dtype, num_splits;
-  bool fp8;  // caches hold OCP e4m3fn
+  bool fp8;  // caches hold one byte an element (OCP e4m3fn, or `rows`)
+  int rows;  // kRowsE4m3 or kRowsInt8: 8-bit rows with a scale each; 0: none
+  const float *ks_rows, *vs_rows;      // their scales [page][head][token]
+  int64_t ks_sp, ks_sh, vs_sp, vs_sh;  // and strides (page, head), elements
   const float *k_scale, *v_scale;
   int ql;      // query tokens per sequence
   int causal;  // bottom-right aligned causal mask
@@ -210,6 +250,10 @@ static int check_call_args(const SplitArgs &a) {
   if (((uintptr_t)a.k_scale & 3u) || ((uintptr_t)a.v_scale & 3u) || ((uintptr_t)a.sinks & 3u) ||
       ((uintptr_t)a.alibi & 3u))
     return MXFA_EINVAL;
+  if (a.rows && (!a.ks_rows || !a.vs_rows || ((uintptr_t)a.ks_rows & 3u) ||
+                 ((uintptr_t)a.vs_rows & 3u) || a.ks_sp < 0 || a.ks_sh < 0 || a.vs_sp < 0 ||
+                 a.vs_sh < 0))
+    return MXFA_EINVAL;
   return MXFA_OK;
 }
 
@@ -254,6 +298,12 @@ static DecodeParams make_params(const SplitArgs &a, const Grid &g) {
   p.ws_s = ws ? (int32_t *)((float *)a.ws + w.o_floats + w.lse_floats) : nullptr;
   p.k_scale = a.fp8 ? a.k_scale : nullptr;
   p.v_scale = a.fp8 ? a.v_scale : nullptr;
+  p.ks_rows = a.ks_rows;
+  p.vs_rows = a.vs_rows;
+  p.ks_sp = a.ks_sp;
+  p.ks_sh = a.ks_sh;
+  p.vs_sp = a.vs_sp;
+  p.vs_sh = a.vs_sh;
   p.scale_log2 = a.scale * kLog2e;
   p.seqlen_add = a.seqlen_add;
   p.batch = a.batch;
@@ -298,6 +348,7 @@ static int launch_partial(const SplitArgs &a, hipStream_t st) {
   // through LDS; four per lane is built for plain calls only.
   int ws = wave_scan_per_lane(a.batch);
   if (ws == 4 && !plain_call(p)) ws = 0;
+  if (a.rows) return launch_rows(p, g, a.hd, a.dtype, a.rows, ws == 1, st);
   switch (a.hd) {
     case 64:
       return ws == 1   ? launch_partial_64_ws(p, g, a.dtype, a.fp8, st)
@@ -413,6 +464,9 @@ static SplitArgs split_args(const void *q, int64_t q_stride_b, int64_t q_stride_
   a.fp8 = false;
   a.k_scale = nullptr;
   a.v_scale = nullptr;
+  a.rows = 0;
+  a.ks_rows = a.vs_rows = nullptr;
+  a.ks_sp = a.ks_sh = a.vs_sp = a.vs_sh = 0;
   a.ql = 1;
   a.causal = 0;
   a.window_left = -1;
@@ -446,6 +500,7 @@ static int launch_seq(const SplitArgs &a, hipStream_t st) {
   DecodeParams p = make_params(a, g);
   p.num_ranges = 0;
   const bool each_tile = a.contiguous && a.same_pages < kTile;
+  if (a.rows) return launch_seq_rows(p, a.hd, a.dtype, a.rows, st);
   switch (a.hd) {
     case 64: return launch_seq_64(p, a.dtype, a.fp8, each_tile, st);
     case 128: return launch_seq_128(p, a.dtype, a.fp8, each_tile, st);
@@ -532,7 +587,8 @@ static int run_tokens(SplitArgs a, int64_t q_stride_t, int q_len, int causal, in
                       const float *sinks, float softcap, const float *alibi_slopes,
                       int64_t out_stride_t, int kv_dtype, const float *k_scale,
                       const float *v_scale, bool wide, hipStream_t st) {
-  if (kv_dtype == MXFA_DTYPE_FP8_E4M3) a = fp8_args(a, k_scale, v_scale);
+  if (a.rows) a.fp8 = true;
+  else if (kv_dtype == MXFA_DTYPE_FP8_E4M3) a = fp8_args(a, k_scale, v_scale);
   else if (kv_dtype != a.dtype) return MXFA_EUNSUPPORTED;
   a.q_st = q_stride_t;
   a.o_st = out_stride_t;
@@ -886,6 +942,31 @@ int mxfa_package_contiguous_decode_launch(
       return MXFA_ELAUNCH;
   }
   return run_split(a, true, st);
+}
+
+int mxfa_package_decode_rows_launch(
+    const void *q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h, int q_len,
+    int causal, int window_left, const float *sinks, float softcap, const float *alibi_slopes,
+    const void *k_cache, const void *v_cache, int64_t cache_stride_page,
+    int64_t cache_stride_token, int64_t cache_stride_head, const float *k_scales,
+    int64_t ks_stride_page, int64_t ks_stride_head, const float *v_scales, int64_t vs_stride_page,
+    int64_t vs_stride_head, const int32_t *block_table, int64_t bt_stride, const int32_t *seqlens,
+    int seqlen_add, void *out, int64_t out_stride_b, int64_t out_stride_t, int64_t out_stride_h,
+    void *workspace, size_t workspace_bytes, float scale, int batch, int q_heads, int kv_heads,
+    int head_dim, int page_size, int block_table_width, int num_pages, int dtype, int kv_dtype,
+    int num_splits, void *stream) {
+  if (kv_dtype != MXFA_DTYPE_FP8_E4M3 && kv_dtype != MXFA_PACKAGE_DTYPE_INT8)
+    return MXFA_EUNSUPPORTED;
+  SplitArgs a = split_args(MXFA_SPLIT_ARGS);
+  a.rows = kv_dtype == MXFA_PACKAGE_DTYPE_INT8 ? kRowsInt8 : kRowsE4m3;
+  a.ks_rows = k_scales;
+  a.vs_rows = v_scales;
+  a.ks_sp = ks_stride_page;
+  a.ks_sh = ks_stride_head;
+  a.vs_sp = vs_stride_page;
+  a.vs_sh = vs_stride_head;
+  return run_tokens(a, q_stride_t, q_len, causal, window_left, sinks, softcap, alibi_slopes,
+                    out_stride_t, kv_dtype, nullptr, nullptr, false, (hipStream_t)stream);
 }
 
 int mxfa_package_tokens_per_launch(int q_len, int gq, int columns) {

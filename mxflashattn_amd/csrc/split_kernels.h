@@ -44,6 +44,9 @@
 //          workspace.
 // fp8 (OCP e4m3fn) caches: k_scale folds into the score scale and v_scale into
 // the output normalisation, both read from device memory once per wave.
+// Caches of 8-bit rows with a scale each (e4m3fn or int8, kF8 = kRowsE4m3 or
+// kRowsInt8): a lane's four tokens' scales come with the tile (16 bytes of K's and
+// of V's); ks multiplies the score, vs the weight ahead of P's rounding, in 32 bits.
 //
 // Combine kernel (second launch; the kernel boundary makes the pieces visible
 // across the XCDs' separate L2s): sequences that cross a range end fold their
@@ -82,6 +85,10 @@
 namespace mxfa {
 
 constexpr int kTile = 16;
+// Cache kinds (template argument kF8): 16-bit, e4m3fn with scales of the whole
+// cache, and 8-bit rows with a scale for each token and kv head.
+constexpr int kRowsE4m3 = 2;
+constexpr int kRowsInt8 = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleLog2 = 8.0f;
 // Tile prefix sums live in LDS, (B + 1) int32 next to a few bytes of static
@@ -119,6 +126,9 @@ struct DecodeParams {
   int32_t *ws_s;
   const float *k_scale;  // fp8 caches: dequantisation scales (nullptr: 1)
   const float *v_scale;
+  const float *ks_rows;  // 8-bit rows: their scales [page][head][token], token stride 1
+  const float *vs_rows;
+  int64_t ks_sp, ks_sh, vs_sp, vs_sh;  // strides of the scales' pages and heads, elements
   const float *sinks;    // per query head logit added once to each denominator (nullptr: none)
   float scale_log2;
   float softcap;         // logit soft-capping: s -> softcap * tanh(s / softcap) (0: none)
@@ -364,11 +374,29 @@ struct Fp8Widen<F16> {
   }
 };
 
-// 8 e4m3fn bytes (two words) to 8 elements (one MFMA operand), in byte order.
-template <typename T>
+// Two codes of an 8-bit cache of kind kF8 (bytes 2*Hi, 2*Hi+1 of w) to a packed
+// pair of the element type, exactly (int8: every |code| <= 128 has at most eight
+// significant bits, bf16's and within fp16's).
+template <typename T, int kF8, bool Hi>
+__device__ __forceinline__ uint32_t widen_pair(uint32_t w) {
+  if constexpr (kF8 == kRowsInt8) {
+    const int s = (int)w;
+    const float a = (float)(Hi ? (s << 8) >> 24 : (s << 24) >> 24);
+    const float b = (float)(Hi ? s >> 24 : (s << 16) >> 24);
+    if constexpr (std::is_same_v<T, BF16>)  // the upper halves hold the whole value
+      return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    else
+      return (uint32_t)Elem<T>::narrow(a) | ((uint32_t)Elem<T>::narrow(b) << 16);
+  } else {
+    return Fp8Widen<T>::template pair<Hi>(w);
+  }
+}
+
+// 8 codes (two words) to 8 elements (one MFMA operand), in byte order.
+template <typename T, int kF8>
 __device__ __forceinline__ uint4 widen8(uint32_t w0, uint32_t w1) {
-  return make_uint4(Fp8Widen<T>::template pair<false>(w0), Fp8Widen<T>::template pair<true>(w0),
-                    Fp8Widen<T>::template pair<false>(w1), Fp8Widen<T>::template pair<true>(w1));
+  return make_uint4(widen_pair<T, kF8, false>(w0), widen_pair<T, kF8, true>(w0),
+                    widen_pair<T, kF8, false>(w1), widen_pair<T, kF8, true>(w1));
 }
 
 // 16-bit element j of a V fragment word list, paired from two tokens.
@@ -785,7 +813,7 @@ struct Tile {
 // kEachTile: every tile moves the reference to its own maximum, up or down (by
 // at most kRescaleLog2), so its largest weight is exactly 1 before P is rounded,
 // as in pieces of one tile each.
-template <int HD, int HR, typename T, bool kF8, bool kLanePages, int NBUF, bool kExtras,
+template <int HD, int HR, typename T, int kF8, bool kLanePages, int NBUF, bool kExtras,
           bool kSeq, bool kBalance = false, bool kProbe = false, int kWaveLocal = 0,
           int kValuG = 0, int kGroups = 1, bool kEachTile = false>
 __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32_t *s_tiles,
@@ -799,6 +827,11 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
   constexpr int VD = HD / 16;                // V elements per lane
   constexpr int VB = kF8 ? VD : 2 * VD;      // V bytes per lane and token
   constexpr int U = 4;                       // V tokens per lane (token 4r+u in DPP row r)
+  constexpr bool kRows = kF8 >= kRowsE4m3;   // 8-bit rows with a scale each
+  // PV's element type. A row's scale times a weight may lie below fp16's range:
+  // an fp16 call on such rows holds V as bf16 and P as the sum of two bf16.
+  constexpr bool kSplitP = kRows && std::is_same_v<T, F16>;
+  using TV = std::conditional_t<kSplitP, BF16, T>;
   constexpr int NPG = kLanePages ? 1 + U : 1;
   // 8-byte V slots (128-byte rows): lanes c and c^8 of a row load 16 bytes
   // (slots 2(c&7), 2(c&7)+1) of two tokens each and swap halves, so a tile
@@ -817,7 +850,7 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
   const uint64_t head_off = (uint64_t)kvh * p.sh_bytes;
   float c = p.scale_log2;
   float v_scale = 1.f;
-  if constexpr (kF8) {
+  if constexpr (kF8 != 0) {
     if (p.k_scale) c *= ((ConstF32)p.k_scale)[0];
     if (p.v_scale) v_scale = ((ConstF32)p.v_scale)[0];
   }
@@ -1004,6 +1037,7 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
     Frag<VB> v[kShareV ? 1 : U];  // kShareV: unused
     uint4 vr[kShareV ? 2 : 1];    // kShareV: tokens 4r+2h, 4r+2h+1, 16 bytes each
     uint4 q[kGroups][NCH];
+    uint4 sc[kRows ? 2 : 1];  // kRows: K's and V's scales of tokens 4r..4r+3
     int lpg[NPG];
     Tile d;
   };
@@ -1038,6 +1072,18 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
 #pragma unroll
         for (int u = 0; u < U; ++u) s.v[u].template load_buf<kAuxStream>(rv, v_off[u]);
       }
+      if constexpr (kRows) {
+        // The tile's 16 scales lie in one page; those past the sequence end are
+        // read with them and not used.
+        const int64_t page = clamp_page(d.pg), at = d.tok0 & ps_mask;
+        const int n = d.valid > 0 ? 64 : 0;
+        const __amdgpu_buffer_rsrc_t rks = make_srd(
+            (const char *)(p.ks_rows + page * p.ks_sp + (int64_t)kvh * p.ks_sh + at), n);
+        const __amdgpu_buffer_rsrc_t rvs = make_srd(
+            (const char *)(p.vs_rows + page * p.vs_sp + (int64_t)kvh * p.vs_sh + at), n);
+        s.sc[0] = buf_load16<0>(rks, row * 16);
+        s.sc[1] = buf_load16<0>(rvs, row * 16);
+      }
     } else {
       // Lane pages: every lane addresses its own page; positions past the
       // sequence end were clamped to its last token (their scores are masked).
@@ -1055,6 +1101,20 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
         const uint64_t off = (uint64_t)(uint32_t)clamp_page(s.lpg[1 + u]) * (uint64_t)p.sp_bytes +
                              (uint64_t)(pos & ps_mask) * st + head_off + col * VB;
         s.v[u].load_ptr(p.v + off);
+      }
+      if constexpr (kRows) {
+        uint32_t w[2][U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int pos = d.tok0 + min(4 * row + u, last);
+          const int64_t page = clamp_page(s.lpg[1 + u]);
+          w[0][u] = __float_as_uint(
+              p.ks_rows[page * p.ks_sp + (int64_t)kvh * p.ks_sh + (pos & ps_mask)]);
+          w[1][u] = __float_as_uint(
+              p.vs_rows[page * p.vs_sp + (int64_t)kvh * p.vs_sh + (pos & ps_mask)]);
+        }
+        s.sc[0] = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
+        s.sc[1] = make_uint4(w[1][0], w[1][1], w[1][2], w[1][3]);
       }
     }
   };
@@ -1125,7 +1185,12 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
             dst[j] = make_float4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv,
                                  v[4 * j + 3] * inv);
           if (col == 0)
-            (kSeq ? lds_lse[hh] : p.ws_lse[pbase + hh]) = Dh > 0.f ? Mh + __log2f(Dh) : -INFINITY;
+            // A piece that is NaN (a row without a scale) joins as +inf, which
+            // leaves NaN in the fold.
+            (kSeq ? lds_lse[hh] : p.ws_lse[pbase + hh]) =
+                Dh > 0.f                 ? Mh + __log2f(Dh)
+                : kRows && !(Dh <= 0.f) ? INFINITY
+                                        : -INFINITY;
         }
       });
     });
@@ -1227,10 +1292,11 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
         }
         acc0[0][i] = v;
       });
-    } else if constexpr (kF8) {
+    } else if constexpr (kF8 != 0) {
 #pragma unroll
       for (int mm = 0; mm < NKL; ++mm) {
-        const uint4 ka = widen8<T>(s.k[mm].x, s.k[mm].y), kb = widen8<T>(s.k[mm].z, s.k[mm].w);
+        const uint4 ka = widen8<T, kF8>(s.k[mm].x, s.k[mm].y);
+        const uint4 kb = widen8<T, kF8>(s.k[mm].z, s.k[mm].w);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
           acc0[g] = Mfma<T>::run(ka, qf[g][2 * mm], acc0[g]);
@@ -1252,18 +1318,38 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
                        : kTwoExact && after_first ? second_move
                                                   : kRescaleLog2;
     after_first = (d.flags & kFirst) != 0;
+    // The tokens' scales. A V row without one (NaN: the row held an infinity or a
+    // NaN) takes its token's score along instead, so that it reaches the columns
+    // that see the token and no other (a weight of zero times NaN would).
+    float ksc[4], vsc[4];
+    if constexpr (kRows) {
+      const uint32_t kw[4] = {s.sc[0].x, s.sc[0].y, s.sc[0].z, s.sc[0].w};
+      const uint32_t vw4[4] = {s.sc[1].x, s.sc[1].y, s.sc[1].z, s.sc[1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = __uint_as_float(vw4[i]);
+        const bool whole = fabsf(v) < INFINITY;
+        ksc[i] = whole ? __uint_as_float(kw[i]) : __builtin_nanf("");
+        vsc[i] = whole ? v : 0.f;
+      }
+    }
     uint2 a[kGroups];  // P of each group, packed pairs of the element type
+    uint2 a_lo[kSplitP ? kGroups : 1];  // kSplitP: what the rounding left
     static_for<kGroups>([&](auto gc) {
       constexpr int g = decltype(gc)::value;
       float x[4];
       bool need = false;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = (acc0[g][i] + acc1[g][i]) * c;
+      for (int i = 0; i < 4; ++i) {
+        x[i] = (acc0[g][i] + acc1[g][i]) * c;
+        if constexpr (kRows) x[i] *= ksc[i];
+      }
       if constexpr (kExtras) {
         if (capped) {  // wave-uniform
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            x[i] = cap_out * tanh_exp2((acc0[g][i] + acc1[g][i]) * cap_in);
+            x[i] = cap_out * tanh_exp2((acc0[g][i] + acc1[g][i]) * cap_in *
+                                       (kRows ? ksc[i] : 1.f));
         }
         if (alibi) {  // wave-uniform; after the cap, as FlashAttention applies it
 #pragma unroll
@@ -1311,10 +1397,23 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
       // P rounded to the element type once; the denominator sums the same
       // rounded weights, so the output stays a convex combination of V rows.
       uint16_t ph[4];
+      if constexpr (kRows) {  // the rounded weights carry the rows' scales
+        dsum[g] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ph[i] = PvMfma<T>::round(pr[i]);
-      dsum[g] += (PvMfma<T>::widen(ph[0]) + PvMfma<T>::widen(ph[1])) +
-                 (PvMfma<T>::widen(ph[2]) + PvMfma<T>::widen(ph[3]));
+        for (int i = 0; i < 4; ++i) pr[i] *= vsc[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ph[i] = PvMfma<TV>::round(pr[i]);
+      if constexpr (!kRows)
+        dsum[g] += (PvMfma<T>::widen(ph[0]) + PvMfma<T>::widen(ph[1])) +
+                   (PvMfma<T>::widen(ph[2]) + PvMfma<T>::widen(ph[3]));
+      if constexpr (kSplitP) {
+        uint16_t pl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pl[i] = PvMfma<TV>::round(pr[i] - PvMfma<TV>::widen(ph[i]));
+        a_lo[g] = make_uint2((uint32_t)pl[0] | ((uint32_t)pl[1] << 16),
+                             (uint32_t)pl[2] | ((uint32_t)pl[3] << 16));
+      }
       a[g] = make_uint2((uint32_t)ph[0] | ((uint32_t)ph[1] << 16),
                         (uint32_t)ph[2] | ((uint32_t)ph[3] << 16));
     });
@@ -1346,9 +1445,9 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
     for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int wi = 0; wi < VD / 2; ++wi) {
-        if constexpr (kF8)
-          vw[u][wi] = (wi & 1) ? Fp8Widen<T>::template pair<true>(vt[u][wi >> 1])
-                               : Fp8Widen<T>::template pair<false>(vt[u][wi >> 1]);
+        if constexpr (kF8 != 0)
+          vw[u][wi] = (wi & 1) ? widen_pair<TV, kF8, true>(vt[u][wi >> 1])
+                               : widen_pair<TV, kF8, false>(vt[u][wi >> 1]);
         else
           vw[u][wi] = vt[u][wi];
       }
@@ -1359,7 +1458,10 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
       const uint2 bv = make_uint2(pair_halves(vw[0][wi], vw[1][wi], odd),
                                   pair_halves(vw[2][wi], vw[3][wi], odd));
 #pragma unroll
-      for (int g = 0; g < kGroups; ++g) oacc[g][jb] = PvMfma<T>::run(a[g], bv, oacc[g][jb]);
+      for (int g = 0; g < kGroups; ++g) {
+        oacc[g][jb] = PvMfma<TV>::run(a[g], bv, oacc[g][jb]);
+        if constexpr (kSplitP) oacc[g][jb] = PvMfma<TV>::run(a_lo[g], bv, oacc[g][jb]);
+      }
     }
     if (d.flags & kLast) finalize(d);
   };
@@ -1430,7 +1532,7 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
 
 // kExtras: the call has a sliding window, soft-capping, ALiBi or sinks (the host
 // picks the instantiation; without them the kernel is the plain one).
-template <int HD, int HR, typename T, bool kF8, bool kLanePages, int NBUF, int WAVES,
+template <int HD, int HR, typename T, int kF8, bool kLanePages, int NBUF, int WAVES,
           bool kExtras, int kWaveScan, int kValuG, int kGroups = 1>
 __global__ __launch_bounds__(WAVES * 64, 1) void split_partial_kernel(const int32_t *seqlens,
                                                                         int batch,
@@ -1667,7 +1769,7 @@ __global__ __launch_bounds__(kCombineThreads) void split_combine_kernel(
 // (fp16, HD 64, 8q/2kv, B 4, 500-767 keys; one-token pages 2.45e-4): one
 // reference for a wave's tiles 2.87e-4, one a tile 2.45e-4, in the same time (4
 // dense sequences of 767 keys 15.5 / 15.4 us a call; the split kernel 19.3).
-template <int HD, int HR, typename T, bool kF8, bool kLanePages, int NBUF, int WAVES, int OCC,
+template <int HD, int HR, typename T, int kF8, bool kLanePages, int NBUF, int WAVES, int OCC,
           bool kExtras, bool kEachTile = false>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(OCC)))
 void seq_decode_kernel(const int32_t *seqlens, const int32_t *bt, int64_t bt_stride, int max_len,
@@ -1754,7 +1856,7 @@ void seq_decode_kernel(const int32_t *seqlens, const int32_t *bt, int64_t bt_str
 // Launch shape by the bytes of one K (or V) head row, RB = HD * element size:
 // 64 (fp8 HD 64), 128 (16-bit HD 64, fp8 HD 128), 256 (16-bit HD 128, fp8
 // HD 256) or 512 (16-bit HD 256).
-template <int HD, bool kF8>
+template <int HD, int kF8>
 constexpr int kRowBytes = HD * (kF8 ? 1 : 2);
 
 // Waves per workgroup: one wave per kv head (KH = min(HKV, waves) kv heads per
@@ -1770,7 +1872,7 @@ constexpr int kRowBytes = HD * (kF8 ? 1 : 2);
 // (16-bit HD 64) and 15% (fp8 HD 128) at 8 kv heads; four beat two sub-ranges
 // of eight by 10% at 4 kv heads; two workgroups per CU lose 2-15% everywhere.
 constexpr int kMinWaves = 4;
-template <int HD, bool kF8>
+template <int HD, int kF8>
 constexpr int kMaxWaves = kRowBytes<HD, kF8> <= 128 ? 8 : 4;
 
 inline int waves_for(int row_bytes, int hkv) {
@@ -1792,7 +1894,7 @@ inline Grid grid_for(int hkv, int num_splits, int waves) {
 // Register sets of the tile pipeline: tiles of 128-byte rows are half the
 // bytes of 256-byte ones, so a third set keeps as many bytes in flight per
 // wave; 64-byte rows (fp8 HD 64) take a fourth.
-template <int HD, bool kF8>
+template <int HD, int kF8>
 constexpr int kNbuf = kRowBytes<HD, kF8> <= 64 ? 4 : kRowBytes<HD, kF8> <= 128 ? 3 : 2;
 
 // Eight-wave workgroups of 128-byte rows (two waves per SIMD) take two
@@ -1805,13 +1907,13 @@ constexpr int kNbuf = kRowBytes<HD, kF8> <= 64 ? 4 : kRowBytes<HD, kF8> <= 128 ?
 // cell (84 tiles) 108.62 / 109.19. Four-wave workgroups (one wave per SIMD)
 // keep three sets everywhere (GQ8 HD64 33.76 / 34.26 with two).
 constexpr int kShortRangeTiles = 64;
-template <int HD, bool kF8, int WAVES>
+template <int HD, int kF8, int WAVES>
 constexpr bool kTwoSetsShort = kRowBytes<HD, kF8> == 128 && WAVES == 8;
 
 // Rows of the MFMA layout that hold used columns (4 columns per row).
 inline int head_rows(int cols) { return cols <= 4 ? 1 : cols <= 8 ? 2 : 4; }
 
-template <int HD, int HR, typename T, bool kF8, int WAVES, bool kExtras, int kWaveScan,
+template <int HD, int HR, typename T, int kF8, int WAVES, bool kExtras, int kWaveScan,
           int kValuG>
 static int launch_partial_s(const DecodeParams &p, const Grid &g, hipStream_t st) {
   dim3 grid(g.gx, g.gy);
@@ -1826,7 +1928,14 @@ static int launch_partial_s(const DecodeParams &p, const Grid &g, hipStream_t st
         return hipGetLastError() == hipSuccess ? MXFA_OK : MXFA_ELAUNCH;
       }
     }
-    hipLaunchKernelGGL((split_partial_kernel<HD, HR, T, kF8, false, kNbuf<HD, kF8>, WAVES, kExtras,
+    // Rows with a scale each: a set holds their scales too, and with options or
+    // fp16's split weights a third set of 128-byte rows does not fit two waves per
+    // SIMD.
+    constexpr int kSets = kF8 >= kRowsE4m3 && kRowBytes<HD, kF8> == 128 &&
+                                  (kExtras || std::is_same_v<T, F16>)
+                              ? 2
+                              : kNbuf<HD, kF8>;
+    hipLaunchKernelGGL((split_partial_kernel<HD, HR, T, kF8, false, kSets, WAVES, kExtras,
                                              kWaveScan, kValuG>),
                        grid, dim3(WAVES * 64), lds, st, p.seqlens, p.batch, p);
   } else {  // per-lane page ids: QK stays on the matrix cores
@@ -1850,7 +1959,7 @@ inline bool plain_call(const DecodeParams &p) {
 // kWaveScan (the wave-local tile scan, 1 or 4 sequences per lane, or 0) is
 // the caller's choice (wave_scan_per_lane, plain_call); the three compile in
 // separate units.
-template <int HD, int HR, typename T, bool kF8, int WAVES, int kWaveScan, int kValuG>
+template <int HD, int HR, typename T, int kF8, int WAVES, int kWaveScan, int kValuG>
 static int launch_partial_w(const DecodeParams &p, const Grid &g, hipStream_t st) {
   const bool extras = p.window_left >= 0 || p.softcap > 0.f || p.sinks || p.alibi;
   if constexpr (kWaveScan == 4) {
@@ -1865,7 +1974,7 @@ static int launch_partial_w(const DecodeParams &p, const Grid &g, hipStream_t st
 // The kernel is the grid's wave count; a grid the instantiations cannot run
 // (more waves than the row size has, or its heads and sub-ranges past the
 // waves) is refused: its extra kv heads would go uncomputed.
-template <int HD, int HR, typename T, bool kF8, int kWaveScan, int kValuG = 0>
+template <int HD, int HR, typename T, int kF8, int kWaveScan, int kValuG = 0>
 static int launch_partial_t(const DecodeParams &p, const Grid &g, hipStream_t st) {
   if (g.heads_per_wg * g.subs > g.waves) return MXFA_ELAUNCH;
   if constexpr (kMaxWaves<HD, kF8> == 8) {
@@ -1900,7 +2009,7 @@ inline int valu_qk_columns(int cols, int hd) {
   return 0;
 }
 
-template <int HD, typename T, bool kF8, int kWaveScan>
+template <int HD, typename T, int kF8, int kWaveScan>
 static int launch_partial_hr(const DecodeParams &p, const Grid &g, hipStream_t st) {
   const int cols = p.gq * p.ql;
   switch (head_rows(cols)) {
@@ -1921,6 +2030,19 @@ static int launch_partial_hr(const DecodeParams &p, const Grid &g, hipStream_t s
     case 2: return launch_partial_t<HD, 2, T, kF8, kWaveScan>(p, g, st);
     default: return launch_partial_t<HD, 4, T, kF8, kWaveScan>(p, g, st);
   }
+}
+
+// The split kernel over 8-bit rows with a scale each, for one head dim and type
+// of q (split_hd*_rows_*.hip): kind kRowsE4m3 or kRowsInt8; the tile scan inside
+// each wave (up to one sequence a lane) or through LDS.
+template <int HD, typename T>
+int launch_rows_hd(const DecodeParams &p, const Grid &g, int kind, bool wave_scan,
+                   hipStream_t st) {
+  if (kind == kRowsE4m3)
+    return wave_scan ? launch_partial_hr<HD, T, kRowsE4m3, 1>(p, g, st)
+                     : launch_partial_hr<HD, T, kRowsE4m3, 0>(p, g, st);
+  return wave_scan ? launch_partial_hr<HD, T, kRowsInt8, 1>(p, g, st)
+                   : launch_partial_hr<HD, T, kRowsInt8, 0>(p, g, st);
 }
 
 // Partial kernel for one head dim: dtype of q/out (MXFA_DTYPE_F16/BF16), fp8
@@ -1952,7 +2074,7 @@ int launch_partial_hd(const DecodeParams &p, const Grid &g, int dtype, bool fp8,
 // (79 us for 8 tokens, 73 for 5); past that, and at head dim 64, each group's
 // softmax and matrix instructions show, since one wave per SIMD has nothing to
 // hide them behind.
-template <int HD, bool kF8, bool kExtras>
+template <int HD, int kF8, bool kExtras>
 constexpr int kMostGroups = HD > 128 ? 1 : kF8 ? 2 : HD == 64 ? 4 : kExtras ? 2 : 3;
 
 // Columns one launch takes: page-uniform tiles (page size >= 16), else 16.
@@ -1964,7 +2086,7 @@ inline int launch_columns(int hd, int ps, bool fp8, bool extras) {
                         : kMostGroups<128, false, false>);
 }
 
-template <int HD, typename T, bool kF8, bool kExtras, int kWaveScan, int kGroups>
+template <int HD, typename T, int kF8, bool kExtras, int kWaveScan, int kGroups>
 static int launch_wide_g(const DecodeParams &p, const Grid &g, hipStream_t st) {
   const size_t lds = kWaveScan ? 0 : (size_t)(p.batch + 1) * sizeof(int32_t);
   hipLaunchKernelGGL((split_partial_kernel<HD, 4, T, kF8, false, kNbuf<HD, kF8>, 4, kExtras,
@@ -1973,7 +2095,7 @@ static int launch_wide_g(const DecodeParams &p, const Grid &g, hipStream_t st) {
   return hipGetLastError() == hipSuccess ? MXFA_OK : MXFA_ELAUNCH;
 }
 
-template <int HD, typename T, bool kF8, bool kExtras, int kWaveScan>
+template <int HD, typename T, int kF8, bool kExtras, int kWaveScan>
 static int launch_wide_s(const DecodeParams &p, const Grid &g, hipStream_t st) {
   constexpr int kMost = kMostGroups<HD, kF8, kExtras>;
   if constexpr (kMost > 2) {
@@ -1984,7 +2106,7 @@ static int launch_wide_s(const DecodeParams &p, const Grid &g, hipStream_t st) {
 
 // Plain calls of up to kWaveScanMax1 sequences scan the tiles inside each
 // wave; the others take the LDS scan (fewer instantiations).
-template <int HD, typename T, bool kF8>
+template <int HD, typename T, int kF8>
 static int launch_wide_x(const DecodeParams &p, const Grid &g, hipStream_t st) {
   if (!plain_call(p)) return launch_wide_s<HD, T, kF8, true, 0>(p, g, st);
   if (wave_scan_per_lane(p.batch) == 1) return launch_wide_s<HD, T, kF8, false, 1>(p, g, st);
@@ -2020,7 +2142,7 @@ inline size_t seq_lds_bytes(int hd, int cols) {
 }
 constexpr size_t kSeqLdsMax = (size_t)64 << 10;
 
-template <int HD, int HR, typename T, bool kF8, bool kExtras>
+template <int HD, int HR, typename T, int kF8, bool kExtras>
 static void launch_seq_x(const DecodeParams &p, hipStream_t st) {
   // The kernel assumes one kv head per workgroup and kSeqWaves waves on it.
   dim3 grid(p.hkv, p.batch);
@@ -2037,7 +2159,7 @@ static void launch_seq_x(const DecodeParams &p, hipStream_t st) {
                        p.max_len, p.seqlen_add, p.ps_log2, p);
 }
 
-template <int HD, int HR, typename T, bool kF8>
+template <int HD, int HR, typename T, int kF8>
 static int launch_seq_t(const DecodeParams &p, hipStream_t st) {
   if (p.window_left >= 0 || p.softcap > 0.f || p.sinks || p.alibi)
     launch_seq_x<HD, HR, T, kF8, true>(p, st);
@@ -2066,7 +2188,7 @@ static int launch_seq_each_hr(const DecodeParams &p, hipStream_t st) {
   }
 }
 
-template <int HD, typename T, bool kF8>
+template <int HD, typename T, int kF8>
 static int launch_seq_hr(const DecodeParams &p, hipStream_t st) {
   switch (head_rows(p.gq * p.ql)) {
     case 1: return launch_seq_t<HD, 1, T, kF8>(p, st);
@@ -2087,6 +2209,13 @@ int launch_seq_hd(const DecodeParams &p, int dtype, bool fp8, bool each_tile, hi
   if (dtype == MXFA_DTYPE_BF16)
     return fp8 ? launch_seq_hr<HD, BF16, true>(p, st) : launch_seq_hr<HD, BF16, false>(p, st);
   return fp8 ? launch_seq_hr<HD, F16, true>(p, st) : launch_seq_hr<HD, F16, false>(p, st);
+}
+
+template <int HD, typename T>
+int launch_seq_rows_hd(const DecodeParams &p, int kind, hipStream_t st) {
+  if (p.heads_per_wg != 1 || p.subs != kSeqWaves) return MXFA_ELAUNCH;  // the kernel's shape
+  return kind == kRowsE4m3 ? launch_seq_hr<HD, T, kRowsE4m3>(p, st)
+                           : launch_seq_hr<HD, T, kRowsInt8>(p, st);
 }
 
 // Streaming probe launch (16-bit caches, page size >= 16): the decode

@@ -50,6 +50,10 @@ DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
 DTYPE_FP8_E4M3 = 2
 # OCP e4m3fn, the fp8 format of gfx950 (MI300's e4m3fnuz is a different code).
 FP8_DTYPE = torch.float8_e4m3fn
+# 8-bit caches with one scale for each token and kv head: their codes (the C
+# side's MXFA_PACKAGE_DTYPE_INT8 for int8).
+DTYPE_INT8 = 3
+ROW_DTYPES = {torch.float8_e4m3fn: DTYPE_FP8_E4M3, torch.int8: DTYPE_INT8}
 
 # The reference's decode contract (vllm_plugin.py:220-261 hands other shapes
 # back); the guards that mirror the reference use these.
@@ -155,6 +159,25 @@ _PACKAGE_SIGNATURES = {
     "mxfa_package_num_splits": (_i, [*[_i] * 10, _p]),
     "mxfa_package_decode_tokens_launch": (
         _i, [*_SIGNATURES["mxfa_split_decode_multi_launch"][1][:-1], _p, _i, _p]),
+    "mxfa_package_decode_rows_launch": (
+        _i,
+        [_p, _i64, _i64, _i64, _i, _i, _i, _p, _f, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64,
+         _p, _i64, _i64, _p, _i64, _p, _i, _p, _i64, _i64, _i64, _p, _sz, _f, _i, _i, _i, _i, _i,
+         _i, _i, _i, _i, _i, _p]),
+    "mxfa_package_prefill_workspace_size": (_i, [_i] * 8 + [ctypes.POINTER(_sz)]),
+    "mxfa_package_prefill_launch": (
+        _i,
+        [_p, _i64, _i64, _i, _p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p,
+         _p, _i64, _p, _p, _i64, _i64, _p, _sz, _f, _i, _i, _f, _p, _p, _i, _i, _i, _i, _i, _i, _i,
+         _i, _i, _i, _p]),
+    "mxfa_package_quantize_and_cache_launch": (
+        _i,
+        [_p, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i, _i,
+         _i, _i, _i, _i, _i, _p]),
+    "mxfa_package_gather_cache_launch": (
+        _i,
+        [_p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _p, _p,
+         _i64, _i64, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
 }
 
 _load_lock = threading.Lock()
@@ -381,8 +404,10 @@ def _require_device(*tensors: torch.Tensor) -> torch.device:
 
 
 def check_decode_shapes(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                        causal: bool = False) -> None:
-    """Raise UnsupportedConfig when the kernel contract does not cover the call."""
+                        causal: bool = False, rows: bool = False) -> None:
+    """Raise UnsupportedConfig when the kernel contract does not cover the call.
+    rows: an 8-bit cache with a scale for each token and kv head (float8_e4m3fn or
+    int8)."""
     if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[1] < 1):
         raise UnsupportedConfig(f"q must be [B,QL,HQ,HD] or [B,HQ,HD], got {tuple(q.shape)}")
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
@@ -399,7 +424,8 @@ def check_decode_shapes(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                                 "(causal calls run in token chunks)")
     if q.dtype not in DTYPE_CODES:
         raise UnsupportedConfig("q must be float16 or bfloat16")
-    if v_cache.dtype != k_cache.dtype or k_cache.dtype not in (q.dtype, FP8_DTYPE):
+    if v_cache.dtype != k_cache.dtype or (k_cache.dtype not in ROW_DTYPES if rows else
+                                          k_cache.dtype not in (q.dtype, FP8_DTYPE)):
         raise UnsupportedConfig("caches must share q's dtype or both be float8_e4m3fn")
     ps = k_cache.shape[1]
     if ps <= 0 or ps & (ps - 1) or ps > 4096:
@@ -510,6 +536,31 @@ def _scale_ptr(scale, device: torch.device, name: str) -> int:
     return _SCALARS.ptr(float(scale), device, name)
 
 
+def has_row_scales(cache: torch.Tensor, *scales) -> bool:
+    """Whether the call's scales are one for each token and kv head: always for int8
+    codes, for float8_e4m3fn where a scale is a rank-3 tensor of more than one value."""
+    if cache.dtype == torch.int8:
+        return True
+    return cache.dtype == FP8_DTYPE and any(
+        isinstance(s, torch.Tensor) and s.dim() == 3 and s.numel() > 1
+        and any(st != 0 for st in s.stride()) for s in scales)
+
+
+def _row_scales(scale, cache: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """Address and strides (page, head) of the scales of a paged 8-bit cache's rows:
+    float32 [pages, kv_heads, page_size] on the cache's GPU, tokens consecutive."""
+    pages, ps, hkv = cache.shape[:3]
+    if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32 or (
+            scale.device != cache.device):
+        raise ValueError(f"{name} must be a float32 tensor on {cache.device}")
+    if scale.shape != (pages, hkv, ps) or (ps > 1 and scale.stride(2) != 1) or (
+            min(scale.stride()) < 0):
+        raise UnsupportedConfig(f"{name} must be [pages, kv_heads, page_size] = "
+                                f"[{pages}, {hkv}, {ps}] with consecutive tokens, or one "
+                                "per-tensor scale of a float8_e4m3fn cache")
+    return scale.data_ptr(), scale.stride(0), scale.stride(1)
+
+
 def token_chunks(q_len: int, per_launch: int, seqlen_add: int) -> list[tuple[int, int, int]]:
     """(first, end, seqlen_add) of each launch of a causal query of q_len tokens
     when one launch holds per_launch tokens. Tokens [first, end) run as the
@@ -522,9 +573,10 @@ def token_chunks(q_len: int, per_launch: int, seqlen_add: int) -> list[tuple[int
     return out
 
 
-def _prepare(q, k_cache, v_cache, block_table, cache_seqlens, out, causal: bool = False):
+def _prepare(q, k_cache, v_cache, block_table, cache_seqlens, out, causal: bool = False,
+             rows: bool = False):
     q, block_table, cache_seqlens = _prepare_inputs(q, k_cache, v_cache, block_table,
-                                                    cache_seqlens, causal)
+                                                    cache_seqlens, causal, rows)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
@@ -536,8 +588,9 @@ def _prepare(q, k_cache, v_cache, block_table, cache_seqlens, out, causal: bool 
     return q, block_table, cache_seqlens, out
 
 
-def _prepare_inputs(q, k_cache, v_cache, block_table, cache_seqlens, causal: bool = False):
-    check_decode_shapes(q, k_cache, v_cache, causal)
+def _prepare_inputs(q, k_cache, v_cache, block_table, cache_seqlens, causal: bool = False,
+                    rows: bool = False):
+    check_decode_shapes(q, k_cache, v_cache, causal, rows)
     batch = q.shape[0]
     hd = q.shape[-1]
     if q.stride(-1) != 1 or (q.shape[-2] > 1 and q.stride(-2) < hd) or (
@@ -659,7 +712,10 @@ def paged_decode_split(
     reading its sequences' keys again);
     caches: [pages, PS, HKV, HD] of q's dtype, or float8_e4m3fn with the
     per-tensor dequantisation scales k_scale / v_scale (float32 device scalars
-    for graph capture); block_table: int32 [B, W]; cache_seqlens: int32 [B].
+    for graph capture), or float8_e4m3fn or int8 codes with a scale for each
+    token and kv head (k_scale / v_scale float32 [pages, HKV, PS], as
+    quantize_and_cache writes them; a scale that is not finite makes the rows
+    that see its key NaN); block_table: int32 [B, W]; cache_seqlens: int32 [B].
     The attended length of sequence b is cache_seqlens[b] + seqlen_add.
     window_left >= 0: sliding window, the token at position i sees keys
     >= i - window_left (FlashAttention's window_size (window_left, 0) with
@@ -673,6 +729,11 @@ def paged_decode_split(
     the one-launch per-sequence kernel (default: split_heuristic, which picks
     the latter for batches of short sequences by the block table's capacity).
     """
+    if has_row_scales(k_cache, k_scale, v_scale):
+        return _paged_decode_rows(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale,
+                                  out, num_splits, int(seqlen_add), k_scale, v_scale,
+                                  bool(causal), int(window_left), sinks, float(softcap),
+                                  alibi_slopes)
     if USE_TORCH_OP:
         # The operator takes the common calls (one 16-bit token, then the
         # general form) and hands any other back as None.
@@ -702,10 +763,7 @@ def paged_decode_split(
             causal=causal, window_left=window_left, sinks=sinks, softcap=softcap,
             alibi_slopes=alibi_slopes)
         return final.copy_(result)
-    if int(window_left) < -1:
-        raise ValueError(f"window_left must be >= -1, got {window_left}")
-    if not (0.0 <= float(softcap) < float("inf")):
-        raise ValueError(f"softcap must be finite and >= 0, got {softcap}")
+    _check_options(window_left, softcap)
     q, block_table, cache_seqlens, out = _prepare(q, k_cache, v_cache, block_table,
                                                   cache_seqlens, out, bool(causal))
     lib = library()
@@ -743,6 +801,164 @@ def paged_decode_split(
         rc = lib.mxfa_split_decode_launch(*args)
         _check(rc, "mxfa_split_decode_launch")
     return out
+
+
+def _check_options(window_left: int, softcap: float) -> None:
+    if int(window_left) < -1:
+        raise ValueError(f"window_left must be >= -1, got {window_left}")
+    if not (0.0 <= float(softcap) < float("inf")):
+        raise ValueError(f"softcap must be finite and >= 0, got {softcap}")
+
+
+def _paged_decode_rows(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale, out,
+                       num_splits, seqlen_add, k_scale, v_scale, causal, window_left, sinks,
+                       softcap, alibi_slopes) -> torch.Tensor:
+    """paged_decode_split over an 8-bit cache with a scale for each token and kv head."""
+    _check_options(window_left, softcap)
+    final = out
+    if out is not None and (out.data_ptr() % 8 or any(st % 4 for st in out.stride()[:-1])):
+        out = None  # the kernels store 8-byte pieces: through a packed copy
+    q, block_table, cache_seqlens, out = _prepare(q, k_cache, v_cache, block_table,
+                                                  cache_seqlens, out, causal, True)
+    ks, vs = _row_scales(k_scale, k_cache, "k_scale"), _row_scales(v_scale, v_cache, "v_scale")
+    ql, hq, hd = (q.shape[1] if q.dim() == 4 else 1), q.shape[-2], q.shape[-1]
+    batch, pages, ps, hkv = q.shape[0], *k_cache.shape[:3]
+    gq = hq // hkv
+    if num_splits is None:
+        num_splits = _num_splits(batch, ql, hq, hkv, hd, ps, block_table.shape[1], 1,
+                                 KERNEL_COLUMNS, num_cus(q.device.index or 0))
+    per_launch = tokens_per_launch(ql, gq, KERNEL_COLUMNS)
+    stream = _stream_handle(q.device)
+    ws_bytes = workspace_size(batch, hq * per_launch, hd, num_splits)
+    ws = WORKSPACE.get(q.device, stream, ws_bytes)
+    _poison(out)
+    q4, o4 = (q, out) if q.dim() == 4 else (q.unsqueeze(1), out.unsqueeze(1))
+    cs = k_cache.stride()
+    for first, end, add in token_chunks(ql, per_launch, seqlen_add):
+        _poison(None, ws)
+        qc, oc = q4[:, first:end], o4[:, first:end]
+        qs, os_ = qc.stride(), oc.stride()
+        rc = library().mxfa_package_decode_rows_launch(
+            qc.data_ptr(), qs[0], qs[1], qs[2], end - first, int(causal), window_left,
+            _sinks_ptr(sinks, q), softcap, _sinks_ptr(alibi_slopes, q, "alibi_slopes"),
+            k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], *ks, *vs,
+            block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), add,
+            oc.data_ptr(), os_[0], os_[1], os_[2], ws.data_ptr(), ws_bytes, float(softmax_scale),
+            batch, hq, hkv, hd, ps, block_table.shape[1], pages, DTYPE_CODES[q.dtype],
+            ROW_DTYPES[k_cache.dtype], num_splits, stream)
+        _check(rc, "mxfa_package_decode_rows_launch")
+    if final is not None and final is not out:
+        return final.copy_(out)
+    return out
+
+
+def paged_prefill(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    block_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    softmax_scale: float,
+    *,
+    causal: bool = True,
+    window_left: int = -1,
+    softcap: float = 0.0,
+    sinks: torch.Tensor | None = None,
+    alibi_slopes: torch.Tensor | None = None,
+    k_scale: torch.Tensor | float | None = None,
+    v_scale: torch.Tensor | float | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of a chunk of new tokens over a paged cache, on the current stream.
+
+    q: [T, HQ, HD], the new tokens of all sequences end to end: rows
+    cu_seqlens_q[b] to cu_seqlens_q[b + 1] (int32 [B + 1], not decreasing) belong to
+    sequence b, any number of them (none, one, a whole prompt). Its
+    cache_seqlens[b] keys, those of the new tokens among them, lie in the pages of
+    block_table[b] (int32 [B, W]); its n new tokens sit at the last n positions, and
+    ``causal`` hides the keys after each. The caches and their scales, window_left,
+    softcap, sinks and alibi_slopes are as in paged_decode_split.
+    Returns ``out`` shaped like q; a token that sees no key gets zeros, and rows
+    that belong to no sequence (behind the last one, in a padded batch) are left as
+    they were.
+
+    The keys' lengths are read on the device: nothing here synchronises, and a
+    captured call replays with other lengths and offsets. Values of keys that a
+    token does not see must be finite where 16 bits hold them and they lie before
+    the sequence's end (a weight of zero times a NaN is a NaN); beyond the end
+    anything may lie.
+    """
+    if q.dim() != 3:
+        raise UnsupportedConfig(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
+    _check_options(window_left, softcap)
+    rows = has_row_scales(k_cache, k_scale, v_scale)
+    check_decode_shapes(q, k_cache, v_cache, True, rows)
+    total, hq, hd = q.shape
+    pages, ps, hkv = k_cache.shape[:3]
+    if k_cache.stride(-1) != 1 or v_cache.stride() != k_cache.stride():
+        raise UnsupportedConfig("k_cache and v_cache must share strides with a contiguous last dim")
+    _require_device(q, k_cache, v_cache, cu_seqlens_q, block_table, cache_seqlens)
+    cu_seqlens_q = _int32_contig(cu_seqlens_q, "cu_seqlens_q")
+    block_table = _int32_contig(block_table, "block_table")
+    cache_seqlens = _int32_contig(cache_seqlens, "cache_seqlens")
+    batch = cache_seqlens.numel()
+    if cu_seqlens_q.dim() != 1 or cu_seqlens_q.numel() != batch + 1:
+        raise ValueError("cu_seqlens_q must have one entry more than cache_seqlens")
+    if batch < 1 or block_table.dim() != 2 or block_table.shape[0] != batch or (
+            block_table.shape[1] < 1):
+        raise ValueError("block_table must be [batch >= 1, width >= 1]")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1
+                            or out.device != q.device):
+        raise ValueError("out must match q's shape, dtype and device with a contiguous last dim")
+    if out is not None and torch._debug_has_internal_overlap(out) == 1:
+        raise ValueError("out must not have internally overlapping memory")
+    final = out
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.data_ptr() % 8 or any(st % 4 for st in out.stride()[:-1]):
+        # Through a packed copy; rows of no sequence keep what they hold.
+        out = final.clone(memory_format=torch.contiguous_format)
+    if q.stride(-1) != 1 or q.data_ptr() % 16 or any(s % 8 for s in q.stride()[:-1]):
+        q = q.clone(memory_format=torch.contiguous_format)
+    ks, vs = (0, 0, 0), (0, 0, 0)
+    k_one = v_one = 0
+    if rows:
+        ks, vs = _row_scales(k_scale, k_cache, "k_scale"), _row_scales(v_scale, v_cache, "v_scale")
+    elif k_cache.dtype == FP8_DTYPE:
+        k_one = _scale_ptr(k_scale, q.device, "k_scale")
+        v_one = _scale_ptr(v_scale, q.device, "v_scale")
+    stream = _stream_handle(q.device)
+    cus = num_cus(q.device.index or 0)
+    ws_bytes = _prefill_workspace(batch, total, hq, hkv, hd, ps, block_table.shape[1], cus)
+    ws = WORKSPACE.get(q.device, stream, ws_bytes) if ws_bytes else None
+    if final is None:
+        _poison(out, ws)
+    else:
+        _poison(None, ws)
+    cs, code = k_cache.stride(), DTYPE_CODES[q.dtype]
+    rc = library().mxfa_package_prefill_launch(
+        q.data_ptr(), q.stride(0), q.stride(1), total, cu_seqlens_q.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], *ks, *vs, k_one, v_one,
+        block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), out.data_ptr(),
+        out.stride(0), out.stride(1), ws.data_ptr() if ws is not None else 0, ws_bytes,
+        float(softmax_scale), int(bool(causal)), int(window_left), float(softcap),
+        _sinks_ptr(sinks, q), _sinks_ptr(alibi_slopes, q, "alibi_slopes"), batch, hq, hkv, hd, ps,
+        block_table.shape[1], pages, code,
+        ROW_DTYPES.get(k_cache.dtype, code), cus, stream)
+    _check(rc, "mxfa_package_prefill_launch")
+    if final is not None and final is not out:
+        return final.copy_(out)
+    return out
+
+
+@functools.lru_cache(maxsize=256)
+def _prefill_workspace(*args: int) -> int:
+    """mxfa_package_prefill_workspace_size of its arguments."""
+    size = _sz()
+    _check(library().mxfa_package_prefill_workspace_size(*args, ctypes.byref(size)),
+           "mxfa_package_prefill_workspace_size")
+    return size.value
 
 
 def paged_decode_split_noalloc(
@@ -984,3 +1200,142 @@ def append_kv(
         _stream_handle(k.device),
     )
     _check(rc, "mxfa_append_kv_launch")
+
+
+def _row_tensors(key: torch.Tensor, value: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """K and V rows as the cache writes read them: shared strides, 16-byte fragments."""
+    if key.stride() != value.stride() or key.stride(-1) != 1 or any(
+            t.data_ptr() % 16 or any(s % 8 for s in t.stride()[:-1]) for t in (key, value)):
+        key = key.clone(memory_format=torch.contiguous_format)
+        value = value.clone(memory_format=torch.contiguous_format)
+    return key, value
+
+
+def quantize_and_cache(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    slot_mapping: torch.Tensor,
+) -> None:
+    """Paged append into an 8-bit cache with a scale for each token and kv head: row t
+    of key/value [tokens, HKV, HD] (float16 or bfloat16) -> slot_mapping[t] (skipped
+    when < 0 or past the cache), codes to the float8_e4m3fn or int8 caches
+    [pages, PS, HKV, HD], scales to k_scale / v_scale (float32 [pages, HKV, PS]).
+
+    In 32 bits: scale = max(max|row| / TOP, 2^-126), TOP 448 (float8_e4m3fn) or 127
+    (int8); code = row / scale to the nearest, ties to even. A row with an infinity or
+    a NaN gets the scale NaN and codes 0, and reads back as NaN. The slots of one call
+    must differ: of two rows with one slot either's codes and either's scale may stay.
+    """
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError("key/value must be [num_tokens, kv_heads, head_dim]")
+    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
+        raise ValueError("caches must be [pages, page_size, kv_heads, head_dim]")
+    if key.shape[1:] != key_cache.shape[2:]:
+        raise ValueError("key/value heads and head_dim must match the cache")
+    if value.dtype != key.dtype or value_cache.dtype != key_cache.dtype or (
+            key_cache.dtype not in ROW_DTYPES):
+        raise ValueError("key/value must share a dtype and the caches be float8_e4m3fn or int8")
+    if value_cache.stride() != key_cache.stride() or key_cache.stride(-1) != 1:
+        raise UnsupportedConfig("caches must share strides with a contiguous last dim")
+    _require_device(key, value, key_cache, value_cache, slot_mapping)
+    ks = _row_scales(k_scale, key_cache, "k_scale")
+    vs = _row_scales(v_scale, value_cache, "v_scale")
+    for name, t in (("caches", key_cache), ("caches", value_cache), ("k_scale", k_scale),
+                    ("v_scale", v_scale)):
+        if torch._debug_has_internal_overlap(t) == 1:
+            raise ValueError(f"{name} must not have internally overlapping memory")
+    key, value = _row_tensors(key, value)
+    slots = slot_mapping.to(torch.int64).contiguous()
+    n = key.shape[0]
+    if slots.dim() != 1 or slots.numel() < n:
+        raise ValueError("slot_mapping must have one entry per token")
+    cs = key_cache.stride()
+    rc = library().mxfa_package_quantize_and_cache_launch(
+        key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), key_cache.data_ptr(),
+        value_cache.data_ptr(), cs[0], cs[1], cs[2], *ks, *vs, slots.data_ptr(), n, key.shape[1],
+        key.shape[2], key_cache.shape[1], key_cache.shape[0], _dtype_code(key),
+        ROW_DTYPES[key_cache.dtype], _stream_handle(key.device))
+    _check(rc, "mxfa_package_quantize_and_cache_launch")
+
+
+def gather_cache(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    total: int,
+    *,
+    k_scale: torch.Tensor | float | None = None,
+    v_scale: torch.Tensor | float | None = None,
+    dtype: torch.dtype | None = None,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached rows of every sequence, packed: the first cu_seqlens[b + 1] -
+    cu_seqlens[b] tokens of sequence b (int32 [B + 1], not decreasing), from the pages
+    of block_table[b], to rows cu_seqlens[b] on of K and V [total, HKV, HD].
+
+    A 16-bit cache is copied bit for bit; an 8-bit one (float8_e4m3fn or int8 with
+    scales as in paged_decode_split) is read back as code * scale in 32 bits, rounded
+    once to ``dtype`` (float16 or bfloat16; with ``out``, its type). Rows of no sequence
+    and those past the block table's row are left as they were (without ``out``:
+    undefined). ``out``: the two tensors to write."""
+    if key_cache.dim() != 4 or value_cache.shape != key_cache.shape or (
+            value_cache.dtype != key_cache.dtype):
+        raise ValueError("caches must be [pages, page_size, kv_heads, head_dim] of one dtype")
+    if value_cache.stride() != key_cache.stride() or key_cache.stride(-1) != 1:
+        raise UnsupportedConfig("caches must share strides with a contiguous last dim")
+    pages, ps, hkv, hd = key_cache.shape
+    _require_device(key_cache, value_cache, block_table, cu_seqlens)
+    device = key_cache.device
+    block_table = _int32_contig(block_table, "block_table")
+    cu_seqlens = _int32_contig(cu_seqlens, "cu_seqlens")
+    if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+        raise ValueError("block_table must be [batch >= 1, width >= 1]")
+    batch = block_table.shape[0]
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() != batch + 1:
+        raise ValueError("cu_seqlens must have one entry more than block_table has rows")
+    total = int(total)
+    if total < 0:
+        raise ValueError(f"total must be >= 0, got {total}")
+    if out is not None:
+        k, v = out
+        for t in (k, v):
+            if t.shape != (total, hkv, hd) or t.device != device or t.stride(-1) != 1 or (
+                    t.dtype != k.dtype):
+                raise ValueError("out must be two tensors [total, kv_heads, head_dim] of one "
+                                 "dtype on the cache's device with a contiguous last dim")
+        if dtype is not None and dtype != k.dtype:
+            raise ValueError("dtype must be out's")
+        if k.stride() != v.stride():
+            raise UnsupportedConfig("out's tensors must share strides")
+        dtype = k.dtype
+    elif dtype is None:
+        dtype = key_cache.dtype
+    if dtype not in DTYPE_CODES:
+        raise UnsupportedConfig(f"dtype {dtype} is not float16/bfloat16")
+    if key_cache.dtype not in (dtype, *ROW_DTYPES):
+        raise UnsupportedConfig("caches must be of the output's dtype, float8_e4m3fn or int8")
+    if out is None:
+        k, v = (torch.empty(total, hkv, hd, dtype=dtype, device=device) for _ in range(2))
+        _poison(k)
+        _poison(v)
+    ks, vs = (0, 0, 0), (0, 0, 0)
+    k_one = v_one = 0
+    if has_row_scales(key_cache, k_scale, v_scale):
+        ks = _row_scales(k_scale, key_cache, "k_scale")
+        vs = _row_scales(v_scale, value_cache, "v_scale")
+    elif key_cache.dtype == FP8_DTYPE:
+        k_one = _scale_ptr(k_scale, device, "k_scale")
+        v_one = _scale_ptr(v_scale, device, "v_scale")
+    cs, code = key_cache.stride(), DTYPE_CODES[dtype]
+    rc = library().mxfa_package_gather_cache_launch(
+        key_cache.data_ptr(), value_cache.data_ptr(), cs[0], cs[1], cs[2], *ks, *vs, k_one, v_one,
+        block_table.data_ptr(), block_table.stride(0), cu_seqlens.data_ptr(), k.data_ptr(),
+        v.data_ptr(), k.stride(0), k.stride(1), batch, block_table.shape[1], total, hkv, hd, ps,
+        pages, code, ROW_DTYPES.get(key_cache.dtype, code), _stream_handle(device))
+    _check(rc, "mxfa_package_gather_cache_launch")
+    return k, v
