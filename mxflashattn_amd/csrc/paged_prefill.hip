@@ -173,6 +173,7 @@ int mxfa_package_prefill_launch(
   p.target = target;
   p.least = kLeastKeys;
   p.max_slots = 2 * target;
+  p.uniform = page_size >= 16 && cache_stride_token * esz < (int64_t)1 << 24;
   char *ws = (char *)workspace;
   if (target) {
     p.ws_o = (float *)(ws + w.o);

@@ -22,8 +22,8 @@
 // A row's maximum is then 31 comparisons in a lane and one swap of the wave's halves.
 //
 // Tiles of 64 keys go through LDS, two buffers each of K and V, rows of HD elements whose
-// 16-byte chunks are permuted within the row (chunk ^ row for K, chunk ^ 2 row for V) so
-// that neither operand read meets a bank conflict. An 8-bit cache is widened exactly on
+// 16-byte chunks are permuted within the row (swizzle_k, swizzle_v) so that neither operand
+// read meets a bank conflict. An 8-bit cache is widened exactly on
 // its way into LDS, once for the whole workgroup; its scales join the scores (ks) and the
 // weights (vs, ahead of P's one rounding) in 32 bits.
 //
@@ -79,12 +79,13 @@ struct PrefillParams {
   int4 *ws_desc;         // [slot][kv head]: pieces (0 but for a tile's first), batch, tile
   int *ws_total;         // slots in use
   int max_slots;
+  int uniform;  // pages of 16 tokens or more (and rows within 32-bit offsets of each other)
 };
 
 // Waves of a workgroup, 32 rows each: eight, two per SIMD; at head dim 256, whose
 // accumulators alone are 128 registers, four with all of a SIMD's registers each.
 template <int HD>
-constexpr int kPrefillWaves = HD == 256 ? 4 : 8;
+constexpr int kPrefillWaves = 4;
 template <int HD>
 constexpr int kPrefillRows = 32 * kPrefillWaves<HD>;
 
@@ -135,6 +136,28 @@ __device__ __forceinline__ uint2 widen_codes(uint32_t w) {
     return make_uint2(Prod32<T>::pack((float)((s << 24) >> 24), (float)((s << 16) >> 24)),
                       Prod32<T>::pack((float)((s << 8) >> 24), (float)(s >> 24)));
   }
+}
+
+// Where row r's 16-byte chunk c lies in an LDS row: c ^ swizzle(r), within each 128 bytes.
+// Eight rows' same K chunk (a b128 read) and four rows' pair of V chunks (a transposed
+// read) then cover all banks once. Rows 8 apart (every pass of the staging) agree.
+__device__ __forceinline__ int swizzle_k(int r) { return r & 7; }
+__device__ __forceinline__ int swizzle_v(int r) { return 2 * (r & 3); }
+
+// Byte offset of a pointer into LDS.
+__device__ __forceinline__ uint32_t lds_offset(const char *ptr) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)ptr;
+}
+
+// 16 bytes a lane from base + off (base the same in the whole wave) to LDS at `lds` + 16 *
+// lane, with no register in between. The compiler does not see the load: the caller waits
+// for it (vmcnt) ahead of the barrier that hands the data over. (The builtin for it makes
+// the compiler wait at the next LDS read, of the other buffer.)
+__device__ __forceinline__ void load_to_lds(const char *base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
 }
 
 // What one sequence asks for: its query rows and keys, held to those that exist.
@@ -248,13 +271,17 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
 }
 
 // One row tile (and piece of its keys) of one kv head.
-template <int HD, typename T, int kCache, bool kExtras>
+//
+// kUniform (pages of 16 tokens or more): the rows that a wave stages at a time lie in one
+// page, so page ids and row addresses are scalars, and a 16-bit cache's rows go to LDS
+// without passing through registers (a lane loads the chunk that belongs where its 16
+// bytes land). Page ids are read a tile ahead of the loads, those a tile ahead of the math.
+template <int HD, typename T, int kCache, bool kExtras, bool kUniform>
 __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(PrefillParams p) {
   constexpr int kThreads = kPrefillWaves<HD> * 64;
   constexpr int kRows = kPrefillRows<HD>;
   constexpr int KT = kPrefillKeys;
   constexpr int kRowBytes = HD * 2;              // of a row in LDS
-  constexpr int kChunks = kRowBytes / 16;        // its 16-byte chunks
   constexpr bool kWide = kCache == kCache16;
   constexpr int kLoadBytes = kWide ? HD * 2 : HD;  // of a row in the cache
   constexpr int kLoads = kLoadBytes / 16;          // its 16-byte loads
@@ -320,79 +347,133 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
   const bool capped = kExtras && p.softcap > 0.f;
   const float slope = kExtras && p.alibi ? p.alibi[kvh * gq + head] * kPrefillLog2e : 0.f;
 
-  // Staging: thread (row, chunk) of each pass.
+  // Staging: thread (row, chunk) of each pass; a wave's rows follow each other.
+  constexpr int kWaveRows = 64 / kLoads;
+  constexpr bool kDirect = kWide && kUniform;
   const int s_row = threadIdx.x / kLoads, s_chunk = threadIdx.x % kLoads;
+  const int w_row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kWaveRows;
   const int ps_mask = (1 << p.ps_log2) - 1;
+  const int last_page = (p.max_len - 1) >> p.ps_log2;
   const int32_t *bt = p.bt + (int64_t)it.b * p.bt_stride;
-  const int64_t head_off = (int64_t)kvh * p.sh + s_chunk * 16;
-  uint4 rk[kPer], rv[kPer];
+  const int64_t head_off = (int64_t)kvh * p.sh;
+  // Byte offsets of this lane from its wave's first row (kUniform).
+  const uint32_t lane_row = (uint32_t)(s_row & (kWaveRows - 1)) * (uint32_t)p.st;
+  const uint32_t k_off =
+      lane_row + (kDirect ? (s_chunk ^ swizzle_k(s_row)) : s_chunk) * 16;
+  const uint32_t v_off =
+      lane_row + (kDirect ? (s_chunk ^ swizzle_v(s_row)) : s_chunk) * 16;
+  uint4 rk[kDirect ? 1 : kPer], rv[kDirect ? 1 : kPer];
   float rks = 0.f, rvs = 0.f;  // 8-bit: the scales of the tile's key threadIdx.x
+  int pg[kPer], pg_scale = 0;  // page ids of the tile to load next
 
-  auto page_of_key = [&](int key) -> int64_t {
-    const int pg = bt[key >> p.ps_log2];
-    return min(max(pg, 0), p.num_pages - 1);
-  };
-  auto load_tile = [&](int j) {
+  // Page ids as the table has them, of keys that may lie past the sequence: the index is
+  // held to the table's row here, the id to the cache where it is used.
+  auto find_pages = [&](int j) {
+    const int key0 = k_begin + j * KT;
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
-      const int r = s_row + u * kPass;
-      const int key = k_begin + j * KT + r;
-      rk[u] = rv[u] = make_uint4(0u, 0u, 0u, 0u);
-      // Rows at or past the sequence's end read as zeros, whatever their memory holds.
-      if (r < KT && key < sq.len) {
-        const int64_t off = page_of_key(key) * p.sp + (int64_t)(key & ps_mask) * p.st + head_off;
+      const int r = u * kPass + (kUniform ? w_row : s_row);
+      const int at = min((key0 + min(r, KT - 1)) >> p.ps_log2, last_page);
+      if constexpr (kUniform)
+        pg[u] = ((const __attribute__((address_space(4))) int32_t *)bt)[at];
+      else
+        pg[u] = bt[at];
+    }
+    if constexpr (!kWide) {
+      if (threadIdx.x < KT) pg_scale = bt[min((key0 + (int)threadIdx.x) >> p.ps_log2, last_page)];
+    }
+  };
+  auto page_off = [&](int page) -> int64_t {
+    return (int64_t)min(max(page, 0), p.num_pages - 1) * p.sp;
+  };
+  auto load_tile = [&](int j, int buf) {
+    const int key0 = k_begin + j * KT;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if constexpr (kUniform) {
+        if (kPass * kPer > KT && u * kPass + w_row >= KT) break;
+        const int64_t off = page_off(pg[u]) +
+                            (int64_t)((key0 + u * kPass + w_row) & ps_mask) * p.st + head_off;
+        if constexpr (kDirect) {
+          const uint32_t at = (u * kPass + w_row) * kRowBytes;
+          load_to_lds(p.k + off, k_off, lds_offset(lds_k[buf]) + at);
+          load_to_lds(p.v + off, v_off, lds_offset(lds_v[buf]) + at);
+        } else {
+          rk[u] = *reinterpret_cast<const uint4 *>(p.k + off + k_off);
+          rv[u] = *reinterpret_cast<const uint4 *>(p.v + off + v_off);
+        }
+      } else {
+        const int r = min(s_row + u * kPass, KT - 1);
+        const int64_t off = page_off(pg[u]) + (int64_t)((key0 + r) & ps_mask) * p.st + head_off +
+                            s_chunk * 16;
         rk[u] = *reinterpret_cast<const uint4 *>(p.k + off);
         rv[u] = *reinterpret_cast<const uint4 *>(p.v + off);
       }
     }
     if constexpr (!kWide) {
       if (threadIdx.x < KT) {
-        const int key = k_begin + j * KT + threadIdx.x;
-        rks = rvs = 0.f;
-        if (key < sq.len) {
-          const int64_t page = page_of_key(key);
-          rks = p.ks ? p.ks[page * p.ks_sp + (int64_t)kvh * p.ks_sh + (key & ps_mask)] : 1.f;
-          rvs = p.vs ? p.vs[page * p.vs_sp + (int64_t)kvh * p.vs_sh + (key & ps_mask)] : 1.f;
-          // A V row without a scale (NaN: it held an infinity or a NaN) takes its key's
-          // score along instead, so that it reaches the rows that see the key and no
-          // other (a weight of zero times NaN would).
-          if (!(fabsf(rvs) < INFINITY)) {
-            rks = __builtin_nanf("");
-            rvs = 0.f;
-          }
-        }
+        const int key = key0 + threadIdx.x;
+        const int64_t page = min(max(pg_scale, 0), p.num_pages - 1);
+        rks = p.ks ? p.ks[page * p.ks_sp + (int64_t)kvh * p.ks_sh + (key & ps_mask)] : 1.f;
+        rvs = p.vs ? p.vs[page * p.vs_sp + (int64_t)kvh * p.vs_sh + (key & ps_mask)] : 1.f;
       }
     }
   };
-  auto store_tile = [&](int buf) {
+  // The tile into LDS (kDirect: it is on its way there; this thread's loads are waited for).
+  // V rows at or past the sequence's end become zeros, whatever their memory holds; their
+  // keys are masked.
+  auto store_tile = [&](int j, int buf) {
+    const int valid = sq.len - (k_begin + j * KT);  // rows of the tile that exist
+    if constexpr (kDirect) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (valid < KT) {
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const int r = s_row + u * kPass;
-      if (kPass * kPer > KT && r >= KT) break;
-      const int sk = r & (kChunks - 1), sv = (2 * r) & (kChunks - 1);
-      char *dk = lds_k[buf] + r * kRowBytes, *dv = lds_v[buf] + r * kRowBytes;
-      if constexpr (kWide) {
-        *reinterpret_cast<uint4 *>(dk + (s_chunk ^ sk) * 16) = rk[u];
-        *reinterpret_cast<uint4 *>(dv + (s_chunk ^ sv) * 16) = rv[u];
-      } else {
-        const uint2 k0 = widen_codes<T, kCache>(rk[u].x), k1 = widen_codes<T, kCache>(rk[u].y);
-        const uint2 k2 = widen_codes<T, kCache>(rk[u].z), k3 = widen_codes<T, kCache>(rk[u].w);
-        const uint2 v0 = widen_codes<TV, kCache>(rv[u].x), v1 = widen_codes<TV, kCache>(rv[u].y);
-        const uint2 v2 = widen_codes<TV, kCache>(rv[u].z), v3 = widen_codes<TV, kCache>(rv[u].w);
-        *reinterpret_cast<uint4 *>(dk + ((2 * s_chunk) ^ sk) * 16) =
-            make_uint4(k0.x, k0.y, k1.x, k1.y);
-        *reinterpret_cast<uint4 *>(dk + ((2 * s_chunk + 1) ^ sk) * 16) =
-            make_uint4(k2.x, k2.y, k3.x, k3.y);
-        *reinterpret_cast<uint4 *>(dv + ((2 * s_chunk) ^ sv) * 16) =
-            make_uint4(v0.x, v0.y, v1.x, v1.y);
-        *reinterpret_cast<uint4 *>(dv + ((2 * s_chunk + 1) ^ sv) * 16) =
-            make_uint4(v2.x, v2.y, v3.x, v3.y);
+        for (int u = 0; u < kPer; ++u) {
+          const int r = s_row + u * kPass;
+          if (r >= valid && r < KT)
+            *reinterpret_cast<uint4 *>(lds_v[buf] + r * kRowBytes + s_chunk * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+        }
       }
-    }
-    if constexpr (!kWide) {
-      if (threadIdx.x < KT) {
-        lds_ks[buf][threadIdx.x] = rks;
-        lds_vs[buf][threadIdx.x] = rvs;
+    } else {
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        const int r = s_row + u * kPass;
+        const uint4 wk = rk[u];
+        const bool there = r < valid;
+        const uint4 wv = make_uint4(there ? rv[u].x : 0u, there ? rv[u].y : 0u,
+                                    there ? rv[u].z : 0u, there ? rv[u].w : 0u);
+        const int sk = swizzle_k(r), sv = swizzle_v(r);
+        if (r < KT) {
+          char *dk = lds_k[buf] + r * kRowBytes, *dv = lds_v[buf] + r * kRowBytes;
+          if constexpr (kWide) {
+            *reinterpret_cast<uint4 *>(dk + (s_chunk ^ sk) * 16) = wk;
+            *reinterpret_cast<uint4 *>(dv + (s_chunk ^ sv) * 16) = wv;
+          } else {
+            const uint2 k0 = widen_codes<T, kCache>(wk.x), k1 = widen_codes<T, kCache>(wk.y);
+            const uint2 k2 = widen_codes<T, kCache>(wk.z), k3 = widen_codes<T, kCache>(wk.w);
+            const uint2 v0 = widen_codes<TV, kCache>(wv.x), v1 = widen_codes<TV, kCache>(wv.y);
+            const uint2 v2 = widen_codes<TV, kCache>(wv.z), v3 = widen_codes<TV, kCache>(wv.w);
+            *reinterpret_cast<uint4 *>(dk + ((2 * s_chunk) ^ sk) * 16) =
+                make_uint4(k0.x, k0.y, k1.x, k1.y);
+            *reinterpret_cast<uint4 *>(dk + ((2 * s_chunk + 1) ^ sk) * 16) =
+                make_uint4(k2.x, k2.y, k3.x, k3.y);
+            *reinterpret_cast<uint4 *>(dv + ((2 * s_chunk) ^ sv) * 16) =
+                make_uint4(v0.x, v0.y, v1.x, v1.y);
+            *reinterpret_cast<uint4 *>(dv + ((2 * s_chunk + 1) ^ sv) * 16) =
+                make_uint4(v2.x, v2.y, v3.x, v3.y);
+          }
+        }
+      }
+      if constexpr (!kWide) {
+        if (threadIdx.x < KT) {
+          // A V row without a scale (NaN: it held an infinity or a NaN) takes its key's score
+          // along instead, so that it reaches the rows that see the key and no other (a
+          // weight of zero times NaN would).
+          const bool whole = fabsf(rvs) < INFINITY;
+          lds_ks[buf][threadIdx.x] = whole ? rks : __builtin_nanf("");
+          lds_vs[buf][threadIdx.x] = whole && (int)threadIdx.x < valid ? rvs : 0.f;
+        }
       }
     }
   };
@@ -415,7 +496,7 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         const uint4 a = *reinterpret_cast<const uint4 *>(
-            base + (((2 * i + half) ^ (r & (kChunks - 1))) * 16));
+            base + (((2 * i + half) ^ swizzle_k(r)) * 16));
         s[kb] = Prod32<T>::run(a, qf[i], s[kb]);
       }
     }
@@ -530,7 +611,7 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
           const int r = st * 16 + 8 * u + v_key;
           const int byte = (d * 32 + v_dim) * 2;
           const int at =
-              r * kRowBytes + ((((byte >> 4) ^ (2 * r)) & (kChunks - 1)) << 4) + (byte & 15);
+              r * kRowBytes + (((byte >> 4) ^ swizzle_v(r)) << 4) + (byte & 15);
           typedef __attribute__((address_space(3))) s16x4v LdsVec;
           const s16x4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec *)(lds_v[buf] + at));
           const uint2 y = __builtin_bit_cast(uint2, x);
@@ -544,12 +625,25 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
     }
   };
 
-  if (j0 < j1) load_tile(j0);
+  if (j0 < j1) {
+    find_pages(j0);
+    load_tile(j0, 0);
+    find_pages(j0 + 1);
+  }
   for (int j = j0; j < j1; ++j) {
     const int buf = (j - j0) & 1;
-    store_tile(buf);
-    if (j + 1 < j1) load_tile(j + 1);
+    // One barrier a tile: past it the tile's rows are there, and every wave is done with
+    // the other buffer, which the next tile's loads then fill.
+    store_tile(j, buf);
+    if (!kDirect && j + 1 < j1) {
+      load_tile(j + 1, buf ^ 1);
+      find_pages(j + 2);
+    }
     __syncthreads();
+    if (kDirect && j + 1 < j1) {
+      load_tile(j + 1, buf ^ 1);
+      find_pages(j + 2);
+    }
     const int key0 = k_begin + j * KT;
     const bool seen = wave_live && key0 <= (p.causal ? pos_hi : sq.len - 1) &&
                       (p.window_left < 0 || key0 + KT - 1 >= pos_lo - p.window_left);
@@ -644,10 +738,14 @@ __global__ __launch_bounds__(kPrefillJoinThreads) void paged_prefill_join_kernel
 template <int HD, typename T, int kCache>
 int launch_prefill_t(const PrefillParams &p, int items, hipStream_t st) {
   const dim3 grid((unsigned)(items * p.hkv)), block(kPrefillWaves<HD> * 64);
-  if (p.softcap > 0.f || p.alibi)
-    hipLaunchKernelGGL((paged_prefill_kernel<HD, T, kCache, true>), grid, block, 0, st, p);
+  const bool extras = p.softcap > 0.f || p.alibi;
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p); };
+  if (p.uniform)
+    extras ? go(paged_prefill_kernel<HD, T, kCache, true, true>)
+           : go(paged_prefill_kernel<HD, T, kCache, false, true>);
   else
-    hipLaunchKernelGGL((paged_prefill_kernel<HD, T, kCache, false>), grid, block, 0, st, p);
+    extras ? go(paged_prefill_kernel<HD, T, kCache, true, false>)
+           : go(paged_prefill_kernel<HD, T, kCache, false, false>);
   if (hipGetLastError() != hipSuccess) return MXFA_ELAUNCH;
   if (p.target == 0) return MXFA_OK;
   hipLaunchKernelGGL((paged_prefill_join_kernel<HD, T>),

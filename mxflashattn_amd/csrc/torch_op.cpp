@@ -11,7 +11,8 @@
 // num_splits None is mxfa_split_heuristic's choice. For any
 // other call it launches nothing and returns None; the Python binding then
 // takes the call and gives its usual errors. decode_tokens (the general call),
-// contiguous_decode, reshape_and_cache and append_kv below do the same.
+// contiguous_decode, reshape_and_cache, append_kv, prefill, quantize_and_cache and
+// gather_cache below do the same.
 //
 // The workspace is grow-only per (device, stream): a buffer replaced by a
 // larger one stays alive until the process ends, since a HIP graph captured
@@ -456,6 +457,56 @@ bool tensor_scale(const c10::optional<at::Tensor> &t, const at::Device &device,
   return true;
 }
 
+// Whether a paged cache is of 8-bit rows with a scale for each token and kv head
+// (native.py's has_row_scales), and then the scales' address and strides (page,
+// head); `ok` false where the kernels do not take them.
+struct RowScales {
+  const float *p = nullptr;
+  int64_t sp = 0, sh = 0;
+};
+
+bool is_row_scale(const c10::optional<at::Tensor> &t) {
+  if (!t.has_value() || t->dim() != 3 || t->numel() <= 1) return false;
+  for (const int64_t st : t->strides())
+    if (st != 0) return true;
+  return false;
+}
+
+bool has_row_scales(const at::Tensor &cache, const c10::optional<at::Tensor> &k_scale,
+                    const c10::optional<at::Tensor> &v_scale) {
+  if (cache.scalar_type() == at::kChar) return true;
+  return cache.scalar_type() == at::kFloat8_e4m3fn &&
+         (is_row_scale(k_scale) || is_row_scale(v_scale));
+}
+
+bool row_scales(const c10::optional<at::Tensor> &t, const at::Tensor &cache, RowScales &s) {
+  if (!t.has_value() || t->scalar_type() != at::kFloat || t->device() != cache.device() ||
+      t->dim() != 3 || t->size(0) != cache.size(0) || t->size(1) != cache.size(2) ||
+      t->size(2) != cache.size(1) || (t->size(2) > 1 && t->stride(2) != 1))
+    return false;
+  s.p = t->data_ptr<float>();
+  s.sp = t->stride(0);
+  s.sh = t->stride(1);
+  return true;
+}
+
+// Paged caches [pages, PS, HKV, HD] of one type and layout with consecutive rows.
+bool cache_pair(const at::Tensor &k, const at::Tensor &v) {
+  return k.dim() == 4 && v.scalar_type() == k.scalar_type() && v.sizes().equals(k.sizes()) &&
+         v.strides().equals(k.strides()) && k.stride(3) == 1 && v.device() == k.device();
+}
+
+// The package's element type codes; -1 for a type the kernels do not take.
+int type_code(at::ScalarType t) {
+  switch (t) {
+    case at::kHalf: return MXFA_DTYPE_F16;
+    case at::kBFloat16: return MXFA_DTYPE_BF16;
+    case at::kFloat8_e4m3fn: return MXFA_DTYPE_FP8_E4M3;
+    case at::kChar: return MXFA_PACKAGE_DTYPE_INT8;
+    default: return -1;
+  }
+}
+
 // decode_tokens(q, k_cache, v_cache, block_table, cache_seqlens, scale, out,
 // num_splits, seqlen_add, causal, window_left, softcap, k_scale, v_scale, sinks,
 // alibi_slopes): the general paged call (several query tokens, fp8 caches,
@@ -474,7 +525,8 @@ py::object decode_tokens(const at::Tensor &q, const at::Tensor &k_cache, const a
                          const c10::optional<at::Tensor> &sinks,
                          const c10::optional<at::Tensor> &alibi_slopes, int64_t advance) {
   const at::ScalarType dt = q.scalar_type();
-  const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  const bool rows = has_row_scales(k_cache, k_scale, v_scale);
+  const bool fp8 = rows || k_cache.scalar_type() == at::kFloat8_e4m3fn;
   if ((dt != at::kHalf && dt != at::kBFloat16) || (!fp8 && k_cache.scalar_type() != dt) ||
       v_cache.scalar_type() != k_cache.scalar_type())
     return py::none();
@@ -511,8 +563,12 @@ py::object decode_tokens(const at::Tensor &q, const at::Tensor &k_cache, const a
   const float *ks, *vs, *sink_ptr, *alibi_ptr;
   if (!head_vector(sinks, hq, device, sink_ptr) || !head_vector(alibi_slopes, hq, device, alibi_ptr))
     return py::none();
-  if (!tensor_scale(fp8 ? k_scale : c10::nullopt, device, ks) ||
-      !tensor_scale(fp8 ? v_scale : c10::nullopt, device, vs))
+  RowScales k_rows, v_rows;
+  if (rows && (advance != 0 || !row_scales(k_scale, k_cache, k_rows) ||
+               !row_scales(v_scale, v_cache, v_rows)))
+    return py::none();
+  if (!tensor_scale(fp8 && !rows ? k_scale : c10::nullopt, device, ks) ||
+      !tensor_scale(fp8 && !rows ? v_scale : c10::nullopt, device, vs))
     return py::none();
   // Strides (batch, token, head); the token stride of one token is not used.
   const auto strides = [&](const at::Tensor &t, int64_t (&s)[3]) {
@@ -539,9 +595,9 @@ py::object decode_tokens(const at::Tensor &q, const at::Tensor &k_cache, const a
   const bool extras = window_left >= 0 || softcap > 0 || sink_ptr || alibi_ptr;
   // Only the entry point of several tokens or options takes shortened sequences;
   // one plain token is refused by the C ABI (mxfa_split_decode_launch).
-  if (seqlen_add < 0 && ql == 1 && !extras) return py::none();
+  if (seqlen_add < 0 && ql == 1 && !extras && !rows) return py::none();
   const int width = (int)block_table.size(1);
-  const int wide = mxfa_package_launch_columns((int)hd, (int)ps, fp8, extras);
+  const int wide = rows ? 16 : mxfa_package_launch_columns((int)hd, (int)ps, fp8, extras);
   int ns = 0;
   if (num_splits_arg.has_value()) {
     const int64_t v = *num_splits_arg;
@@ -569,7 +625,16 @@ py::object decode_tokens(const at::Tensor &q, const at::Tensor &k_cache, const a
     if (t > 0) poison(stream, nullptr, ws_bytes ? &ws_t : nullptr);
     // Tokens [t, t + n) as the last n tokens of sequences shortened by the
     // tokens after them.
-    const int rc = mxfa_package_decode_tokens_launch(
+    const int rc = rows ? mxfa_package_decode_rows_launch(
+        (const char *)q.data_ptr() + t * qs[1] * esz, qs[0], qs[1], qs[2], (int)n, causal,
+        (int)window_left, sink_ptr, (float)softcap, alibi_ptr, k_cache.data_ptr(),
+        v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), k_rows.p,
+        k_rows.sp, k_rows.sh, v_rows.p, v_rows.sp, v_rows.sh, block_table.data_ptr<int32_t>(),
+        block_table.stride(0), cache_seqlens.data_ptr<int32_t>(),
+        (int)(seqlen_add - (ql - t - n)), (char *)out.data_ptr() + t * os[1] * esz, os[0], os[1],
+        os[2], ws, ws_bytes, (float)scale, (int)batch, (int)hq, (int)hkv, (int)hd, (int)ps, width,
+        (int)pages, type_code(dt), type_code(k_cache.scalar_type()), ns, stream)
+    : mxfa_package_decode_tokens_launch(
         (const char *)q.data_ptr() + t * qs[1] * esz, qs[0], qs[1], qs[2], (int)n, causal,
         (int)window_left, sink_ptr, (float)softcap, alibi_ptr, k_cache.data_ptr(),
         v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
@@ -688,6 +753,173 @@ bool append_kv(const at::Tensor &k, const at::Tensor &v, const at::Tensor &k_cac
   return true;
 }
 
+// prefill(q, k_cache, v_cache, cu_seqlens_q, block_table, cache_seqlens, scale, causal,
+// window_left, softcap, sinks, alibi_slopes, k_scale, v_scale, out): paged_prefill for
+// tensors that the kernels read in place (int32 metadata; scales tensors or None). Returns
+// the output, or None (nothing launched) for any other call.
+py::object prefill(const at::Tensor &q, const at::Tensor &k_cache, const at::Tensor &v_cache,
+                   const at::Tensor &cu_seqlens_q, const at::Tensor &block_table,
+                   const at::Tensor &cache_seqlens, double scale, bool causal,
+                   int64_t window_left, double softcap, const c10::optional<at::Tensor> &sinks,
+                   const c10::optional<at::Tensor> &alibi_slopes,
+                   const c10::optional<at::Tensor> &k_scale,
+                   const c10::optional<at::Tensor> &v_scale,
+                   const c10::optional<at::Tensor> &out_arg) {
+  const at::ScalarType dt = q.scalar_type();
+  if ((dt != at::kHalf && dt != at::kBFloat16) || !q.is_cuda() || q.dim() != 3 ||
+      q.stride(2) != 1 || !cache_pair(k_cache, v_cache))
+    return py::none();
+  const at::Device device = q.device();
+  const bool rows = has_row_scales(k_cache, k_scale, v_scale);
+  const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  if ((!rows && !fp8 && k_cache.scalar_type() != dt) || k_cache.device() != device ||
+      device.index() != c10::hip::current_device())
+    return py::none();
+  for (const at::Tensor *t : {&cu_seqlens_q, &cache_seqlens})
+    if (t->scalar_type() != at::kInt || t->dim() != 1 || !t->is_contiguous() ||
+        t->device() != device)
+      return py::none();
+  const int64_t batch = cache_seqlens.size(0), total = q.size(0), hq = q.size(1), hd = q.size(2);
+  const int64_t pages = k_cache.size(0), ps = k_cache.size(1), hkv = k_cache.size(2);
+  const int64_t most = std::numeric_limits<int>::max();
+  if (block_table.scalar_type() != at::kInt || block_table.dim() != 2 ||
+      block_table.device() != device || block_table.stride(1) != 1 || batch < 1 ||
+      block_table.size(0) != batch || block_table.size(1) < 1 || block_table.size(1) > most ||
+      cu_seqlens_q.size(0) != batch + 1 || k_cache.size(3) != hd || total > most ||
+      pages > most || hq > most || hkv < 1 || hq % hkv || ps > 4096 || batch > most)
+    return py::none();
+  if (window_left < -1 || window_left > 1 << 30 || !(softcap >= 0.0) ||
+      softcap == std::numeric_limits<double>::infinity())
+    return py::none();
+  const float *sink_ptr, *alibi_ptr, *ks = nullptr, *vs = nullptr;
+  if (!head_vector(sinks, hq, device, sink_ptr) || !head_vector(alibi_slopes, hq, device, alibi_ptr))
+    return py::none();
+  RowScales k_rows, v_rows;
+  if (rows ? !row_scales(k_scale, k_cache, k_rows) || !row_scales(v_scale, v_cache, v_rows)
+           : !tensor_scale(fp8 ? k_scale : c10::nullopt, device, ks) ||
+                 !tensor_scale(fp8 ? v_scale : c10::nullopt, device, vs))
+    return py::none();
+  if (!aligned(q.data_ptr(), 16) || ((q.stride(0) | q.stride(1)) & 7)) return py::none();
+  at::Tensor out;
+  if (out_arg.has_value()) {
+    out = *out_arg;
+    if (out.scalar_type() != dt || out.device() != device || !out.sizes().equals(q.sizes()) ||
+        out.stride(2) != 1 || !aligned(out.data_ptr(), 8) || ((out.stride(0) | out.stride(1)) & 3))
+      return py::none();
+  } else {
+    out = at::empty(q.sizes(), q.options());
+  }
+  const int cus = num_cus(device.index());
+  size_t ws_bytes = 0;
+  if (mxfa_package_prefill_workspace_size((int)batch, (int)total, (int)hq, (int)hkv, (int)hd,
+                                          (int)ps, (int)block_table.size(1), cus, &ws_bytes) !=
+      MXFA_OK)
+    return py::none();
+  void *stream = (void *)c10::hip::getCurrentHIPStream(device.index()).stream();
+  at::Tensor ws_t;
+  if (ws_bytes) ws_t = workspace(device, stream, ws_bytes);
+  // A given output keeps the rows of no sequence.
+  poison(stream, out_arg.has_value() ? nullptr : &out, ws_bytes ? &ws_t : nullptr);
+  const int rc = mxfa_package_prefill_launch(
+      q.data_ptr(), q.stride(0), q.stride(1), (int)total, cu_seqlens_q.data_ptr<int32_t>(),
+      k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+      k_cache.stride(2), k_rows.p, k_rows.sp, k_rows.sh, v_rows.p, v_rows.sp, v_rows.sh, ks, vs,
+      block_table.data_ptr<int32_t>(), block_table.stride(0), cache_seqlens.data_ptr<int32_t>(),
+      out.data_ptr(), out.stride(0), out.stride(1), ws_bytes ? ws_t.data_ptr() : nullptr, ws_bytes,
+      (float)scale, causal, (int)window_left, (float)softcap, sink_ptr, alibi_ptr, (int)batch,
+      (int)hq, (int)hkv, (int)hd, (int)ps, (int)block_table.size(1), (int)pages, type_code(dt),
+      type_code(k_cache.scalar_type()), cus, stream);
+  if (rc == MXFA_EUNSUPPORTED || rc == MXFA_EINVAL) return py::none();  // nothing launched
+  if (rc != MXFA_OK)
+    throw std::runtime_error(std::string("mxfa_package_prefill_launch failed (") +
+                             std::to_string(rc) + "): " + mxfa_strerror(rc));
+  return py::cast(out);
+}
+
+// quantize_and_cache(key, value, key_cache, value_cache, k_scale, v_scale, slot_mapping) for
+// tensors the kernel reads and writes in place. True once launched, false (nothing launched)
+// for any other call.
+bool quantize_and_cache(const at::Tensor &key, const at::Tensor &value,
+                        const at::Tensor &key_cache, const at::Tensor &value_cache,
+                        const at::Tensor &k_scale, const at::Tensor &v_scale,
+                        const at::Tensor &slot_mapping) {
+  const at::ScalarType codes = key_cache.scalar_type();
+  if ((codes != at::kFloat8_e4m3fn && codes != at::kChar) ||
+      !append_tensors(key, value, key_cache, value_cache, 3, codes))
+    return false;
+  const at::Device device = key.device();
+  const int64_t most = std::numeric_limits<int>::max();
+  if (slot_mapping.scalar_type() != at::kLong || slot_mapping.dim() != 1 ||
+      !slot_mapping.is_contiguous() || slot_mapping.size(0) < key.size(0) ||
+      slot_mapping.device() != device || key.size(0) > most || key_cache.size(0) > most)
+    return false;
+  RowScales ks, vs;
+  if (!row_scales(k_scale, key_cache, ks) || !row_scales(v_scale, value_cache, vs)) return false;
+  for (const at::Tensor *t : {&key_cache, &value_cache, &k_scale, &v_scale})
+    if (at::has_internal_overlap(*t) == at::MemOverlap::Yes) return false;
+  void *stream = (void *)c10::hip::getCurrentHIPStream(device.index()).stream();
+  const int rc = mxfa_package_quantize_and_cache_launch(
+      key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), key_cache.data_ptr(),
+      value_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1), key_cache.stride(2),
+      const_cast<float *>(ks.p), ks.sp, ks.sh, const_cast<float *>(vs.p), vs.sp, vs.sh,
+      slot_mapping.data_ptr<int64_t>(), (int)key.size(0), (int)key.size(1), (int)key.size(2),
+      (int)key_cache.size(1), (int)key_cache.size(0), type_code(key.scalar_type()),
+      type_code(codes), stream);
+  if (rc == MXFA_EUNSUPPORTED || rc == MXFA_EINVAL) return false;  // nothing launched
+  if (rc != MXFA_OK)
+    throw std::runtime_error(std::string("mxfa_package_quantize_and_cache_launch failed (") +
+                             std::to_string(rc) + "): " + mxfa_strerror(rc));
+  return true;
+}
+
+// gather_cache(key_cache, value_cache, block_table, cu_seqlens, total, k_scale, v_scale,
+// bf16) into new tensors of fp16 or bf16, for caches the kernel reads in place. Returns
+// (K, V), or None (nothing launched) for any other call.
+py::object gather_cache(const at::Tensor &key_cache, const at::Tensor &value_cache,
+                        const at::Tensor &block_table, const at::Tensor &cu_seqlens,
+                        int64_t total, const c10::optional<at::Tensor> &k_scale,
+                        const c10::optional<at::Tensor> &v_scale, bool bf16) {
+  const at::ScalarType dt = bf16 ? at::kBFloat16 : at::kHalf;
+  if (!key_cache.is_cuda() || !cache_pair(key_cache, value_cache)) return py::none();
+  const at::Device device = key_cache.device();
+  const bool rows = has_row_scales(key_cache, k_scale, v_scale);
+  const bool fp8 = key_cache.scalar_type() == at::kFloat8_e4m3fn;
+  const int64_t most = std::numeric_limits<int>::max();
+  if ((!rows && !fp8 && key_cache.scalar_type() != dt) ||
+      device.index() != c10::hip::current_device() || block_table.scalar_type() != at::kInt ||
+      block_table.dim() != 2 || block_table.device() != device || block_table.stride(1) != 1 ||
+      block_table.size(0) < 1 || block_table.size(1) < 1 || block_table.size(0) > most ||
+      block_table.size(1) > most || cu_seqlens.scalar_type() != at::kInt ||
+      cu_seqlens.dim() != 1 || cu_seqlens.device() != device || !cu_seqlens.is_contiguous() ||
+      cu_seqlens.size(0) != block_table.size(0) + 1 || total < 0 || total > most ||
+      key_cache.size(0) > most)
+    return py::none();
+  const float *ks = nullptr, *vs = nullptr;
+  RowScales k_rows, v_rows;
+  if (rows ? !row_scales(k_scale, key_cache, k_rows) || !row_scales(v_scale, value_cache, v_rows)
+           : !tensor_scale(fp8 ? k_scale : c10::nullopt, device, ks) ||
+                 !tensor_scale(fp8 ? v_scale : c10::nullopt, device, vs))
+    return py::none();
+  const int64_t hkv = key_cache.size(2), hd = key_cache.size(3);
+  const auto options = key_cache.options().dtype(dt);
+  at::Tensor k = at::empty({total, hkv, hd}, options), v = at::empty({total, hkv, hd}, options);
+  void *stream = (void *)c10::hip::getCurrentHIPStream(device.index()).stream();
+  poison(stream, &k, nullptr);
+  poison(stream, &v, nullptr);
+  const int rc = mxfa_package_gather_cache_launch(
+      key_cache.data_ptr(), value_cache.data_ptr(), key_cache.stride(0), key_cache.stride(1),
+      key_cache.stride(2), k_rows.p, k_rows.sp, k_rows.sh, v_rows.p, v_rows.sp, v_rows.sh, ks, vs,
+      block_table.data_ptr<int32_t>(), block_table.stride(0), cu_seqlens.data_ptr<int32_t>(),
+      k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), (int)block_table.size(0),
+      (int)block_table.size(1), (int)total, (int)hkv, (int)hd, (int)key_cache.size(1),
+      (int)key_cache.size(0), type_code(dt), type_code(key_cache.scalar_type()), stream);
+  if (rc == MXFA_EUNSUPPORTED || rc == MXFA_EINVAL) return py::none();  // nothing launched
+  if (rc != MXFA_OK)
+    throw std::runtime_error(std::string("mxfa_package_gather_cache_launch failed (") +
+                             std::to_string(rc) + "): " + mxfa_strerror(rc));
+  return py::make_tuple(k, v);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_mxfa_torch, m) {
@@ -722,6 +954,17 @@ PYBIND11_MODULE(_mxfa_torch, m) {
         py::arg("k_scale"), py::arg("v_scale"));
   m.def("append_kv", &append_kv, py::arg("k"), py::arg("v"), py::arg("k_cache"),
         py::arg("v_cache"), py::arg("block_table"), py::arg("cache_seqlens"));
+  m.def("prefill", &prefill, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("cu_seqlens_q"), py::arg("block_table"), py::arg("cache_seqlens"),
+        py::arg("scale"), py::arg("causal"), py::arg("window_left"), py::arg("softcap"),
+        py::arg("sinks"), py::arg("alibi_slopes"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("out"));
+  m.def("quantize_and_cache", &quantize_and_cache, py::arg("key"), py::arg("value"),
+        py::arg("key_cache"), py::arg("value_cache"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("slot_mapping"));
+  m.def("gather_cache", &gather_cache, py::arg("key_cache"), py::arg("value_cache"),
+        py::arg("block_table"), py::arg("cu_seqlens"), py::arg("total"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("bf16"));
   m.def("abi_version", &mxfa_abi_version);
   m.def("workspace_bytes", &workspace_bytes,
         "(bytes of live workspaces, bytes of workspaces replaced by larger ones)");

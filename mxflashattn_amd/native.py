@@ -729,11 +729,6 @@ def paged_decode_split(
     the one-launch per-sequence kernel (default: split_heuristic, which picks
     the latter for batches of short sequences by the block table's capacity).
     """
-    if has_row_scales(k_cache, k_scale, v_scale):
-        return _paged_decode_rows(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale,
-                                  out, num_splits, int(seqlen_add), k_scale, v_scale,
-                                  bool(causal), int(window_left), sinks, float(softcap),
-                                  alibi_slopes)
     if USE_TORCH_OP:
         # The operator takes the common calls (one 16-bit token, then the
         # general form) and hands any other back as None.
@@ -753,6 +748,11 @@ def paged_decode_split(
                                           k_scale, v_scale, sinks, alibi_slopes)
             if result is not None:
                 return result if out is None else out
+    if has_row_scales(k_cache, k_scale, v_scale):
+        return _paged_decode_rows(q, k_cache, v_cache, block_table, cache_seqlens, softmax_scale,
+                                  out, num_splits, int(seqlen_add), k_scale, v_scale,
+                                  bool(causal), int(window_left), sinks, float(softcap),
+                                  alibi_slopes)
     if out is not None and (out.data_ptr() % 8 or any(st % 4 for st in out.stride()[:-1])):
         # The kernels store 8-byte pieces of each output row; a view that is
         # not laid out for that gets the result through a packed copy.
@@ -889,6 +889,13 @@ def paged_prefill(
     the sequence's end (a weight of zero times a NaN is a NaN); beyond the end
     anything may lie.
     """
+    op = torch_op() if USE_TORCH_OP and _op_scales(k_scale, v_scale, sinks, alibi_slopes) else None
+    if op is not None:
+        result = op.prefill(q, k_cache, v_cache, cu_seqlens_q, block_table, cache_seqlens,
+                            float(softmax_scale), bool(causal), int(window_left), float(softcap),
+                            sinks, alibi_slopes, k_scale, v_scale, out)
+        if result is not None:
+            return result if out is None else out
     if q.dim() != 3:
         raise UnsupportedConfig(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
     _check_options(window_left, softcap)
@@ -1230,6 +1237,10 @@ def quantize_and_cache(
     a NaN gets the scale NaN and codes 0, and reads back as NaN. The slots of one call
     must differ: of two rows with one slot either's codes and either's scale may stay.
     """
+    op = torch_op() if USE_TORCH_OP and _op_scales(k_scale, v_scale) else None
+    if op is not None and k_scale is not None and v_scale is not None and op.quantize_and_cache(
+            key, value, key_cache, value_cache, k_scale, v_scale, slot_mapping):
+        return
     if key.dim() != 3 or value.shape != key.shape:
         raise ValueError("key/value must be [num_tokens, kv_heads, head_dim]")
     if key_cache.dim() != 4 or value_cache.shape != key_cache.shape:
@@ -1283,6 +1294,12 @@ def gather_cache(
     once to ``dtype`` (float16 or bfloat16; with ``out``, its type). Rows of no sequence
     and those past the block table's row are left as they were (without ``out``:
     undefined). ``out``: the two tensors to write."""
+    op = torch_op() if USE_TORCH_OP and out is None and _op_scales(k_scale, v_scale) else None
+    if op is not None and (dtype or key_cache.dtype) in DTYPE_CODES:
+        result = op.gather_cache(key_cache, value_cache, block_table, cu_seqlens, int(total),
+                                 k_scale, v_scale, (dtype or key_cache.dtype) == torch.bfloat16)
+        if result is not None:
+            return result
     if key_cache.dim() != 4 or value_cache.shape != key_cache.shape or (
             value_cache.dtype != key_cache.dtype):
         raise ValueError("caches must be [pages, page_size, kv_heads, head_dim] of one dtype")
