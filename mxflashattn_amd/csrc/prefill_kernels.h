@@ -98,6 +98,10 @@ template <typename T>
 struct Prod32;
 template <>
 struct Prod32<F16> {
+  static __device__ __forceinline__ float add_pair(uint32_t w, float l) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2v, w),
+                                  __builtin_bit_cast(f16x2v, 0x3c003c00u), l, false);
+  }
   static __device__ __forceinline__ f32x16 run(const uint4 &a, const uint4 &b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -109,6 +113,10 @@ struct Prod32<F16> {
 };
 template <>
 struct Prod32<BF16> {
+  static __device__ __forceinline__ float add_pair(uint32_t w, float l) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2v, w),
+                                           __builtin_bit_cast(bf16x2v, 0x3f803f80u), l, false);
+  }
   static __device__ __forceinline__ f32x16 run(const uint4 &a, const uint4 &b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -138,11 +146,18 @@ __device__ __forceinline__ uint2 widen_codes(uint32_t w) {
   }
 }
 
-// Where row r's 16-byte chunk c lies in an LDS row: c ^ swizzle(r), within each 128 bytes.
-// Eight rows' same K chunk (a b128 read) and four rows' pair of V chunks (a transposed
-// read) then cover all banks once. Rows 8 apart (every pass of the staging) agree.
-__device__ __forceinline__ int swizzle_k(int r) { return r & 7; }
-__device__ __forceinline__ int swizzle_v(int r) { return 2 * (r & 3); }
+// Where row r's 16-byte chunk c lies in its LDS row: c ^ swizzle(r). LDS serves 256 bytes
+// a clock, each 16-byte column of them once: 16 lanes of a b128 read (16 rows' same K chunk)
+// and 32 of a transposed b64 read (four rows' four V chunks) then take a clock each. (With
+// permutations within 128 bytes half of LDS's busy cycles were conflicts.)
+template <int HD>
+__device__ __forceinline__ int swizzle_k(int r) {
+  return HD == 64 ? (r >> 1) & 7 : r & 15;
+}
+template <int HD>
+__device__ __forceinline__ int swizzle_v(int r) {
+  return HD == 64 ? 4 * ((r >> 1) & 1) : 4 * (r & 3);
+}
 
 // Byte offset of a pointer into LDS.
 __device__ __forceinline__ uint32_t lds_offset(const char *ptr) {
@@ -341,8 +356,19 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
     for (int i = 0; i < NQ; ++i)
       qf[i] = live ? *reinterpret_cast<const uint4 *>(src + i * 32) : make_uint4(0u, 0u, 0u, 0u);
   }
+  // Scores are kept as products; c takes them to base 2 in one multiply-add with the
+  // reference. c > 0: a negative scale's sign goes to q, and a scale of zero zeroes q.
   float c = p.scale * kPrefillLog2e;
   if (!kWide && p.k_scale) c *= p.k_scale[0];
+  {
+    const uint32_t keep = c == 0.f ? 0u : 0xffffffffu, flip = c < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+      qf[i] = make_uint4((qf[i].x ^ flip) & keep, (qf[i].y ^ flip) & keep,
+                         (qf[i].z ^ flip) & keep, (qf[i].w ^ flip) & keep);
+    c = c == 0.f ? 1.f : fabsf(c);
+  }
+  const float cs = kExtras ? 1.f : c;  // what is left to multiply scores by at the exponent
   const float v_scale = !kWide && p.v_scale ? p.v_scale[0] : 1.f;
   const bool capped = kExtras && p.softcap > 0.f;
   const float slope = kExtras && p.alibi ? p.alibi[kvh * gq + head] * kPrefillLog2e : 0.f;
@@ -356,12 +382,14 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
   const int last_page = (p.max_len - 1) >> p.ps_log2;
   const int32_t *bt = p.bt + (int64_t)it.b * p.bt_stride;
   const int64_t head_off = (int64_t)kvh * p.sh;
-  // Byte offsets of this lane from its wave's first row (kUniform).
+  // Byte offsets of this lane from its wave's first row (kUniform). A pass of eight rows
+  // (head dim 256) swaps K's chunk halves every other time.
+  static_assert(!kDirect || kPass % 16 == 0 || (HD == 256 && kPass % 8 == 0), "swizzle_k");
   const uint32_t lane_row = (uint32_t)(s_row & (kWaveRows - 1)) * (uint32_t)p.st;
-  const uint32_t k_off =
-      lane_row + (kDirect ? (s_chunk ^ swizzle_k(s_row)) : s_chunk) * 16;
-  const uint32_t v_off =
-      lane_row + (kDirect ? (s_chunk ^ swizzle_v(s_row)) : s_chunk) * 16;
+  const uint32_t k_off = lane_row + (kDirect ? (s_chunk ^ swizzle_k<HD>(s_row)) : s_chunk) * 16;
+  const uint32_t k_off_odd =
+      kPass % 16 == 0 ? k_off : lane_row + (s_chunk ^ swizzle_k<HD>(s_row + kPass)) * 16;
+  const uint32_t v_off = lane_row + (kDirect ? (s_chunk ^ swizzle_v<HD>(s_row)) : s_chunk) * 16;
   uint4 rk[kDirect ? 1 : kPer], rv[kDirect ? 1 : kPer];
   float rks = 0.f, rvs = 0.f;  // 8-bit: the scales of the tile's key threadIdx.x
   int pg[kPer], pg_scale = 0;  // page ids of the tile to load next
@@ -396,7 +424,7 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
                             (int64_t)((key0 + u * kPass + w_row) & ps_mask) * p.st + head_off;
         if constexpr (kDirect) {
           const uint32_t at = (u * kPass + w_row) * kRowBytes;
-          load_to_lds(p.k + off, k_off, lds_offset(lds_k[buf]) + at);
+          load_to_lds(p.k + off, u & 1 ? k_off_odd : k_off, lds_offset(lds_k[buf]) + at);
           load_to_lds(p.v + off, v_off, lds_offset(lds_v[buf]) + at);
         } else {
           rk[u] = *reinterpret_cast<const uint4 *>(p.k + off + k_off);
@@ -443,7 +471,7 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
         const bool there = r < valid;
         const uint4 wv = make_uint4(there ? rv[u].x : 0u, there ? rv[u].y : 0u,
                                     there ? rv[u].z : 0u, there ? rv[u].w : 0u);
-        const int sk = swizzle_k(r), sv = swizzle_v(r);
+        const int sk = swizzle_k<HD>(r), sv = swizzle_v<HD>(r);
         if (r < KT) {
           char *dk = lds_k[buf] + r * kRowBytes, *dv = lds_v[buf] + r * kRowBytes;
           if constexpr (kWide) {
@@ -496,11 +524,11 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         const uint4 a = *reinterpret_cast<const uint4 *>(
-            base + (((2 * i + half) ^ swizzle_k(r)) * 16));
+            base + (((2 * i + half) ^ swizzle_k<HD>(r)) * 16));
         s[kb] = Prod32<T>::run(a, qf[i], s[kb]);
       }
     }
-    // Scores in base 2: keys kb * 32 + 8 (i / 4) + 4 half + i % 4 of the tile.
+    // Scores: keys kb * 32 + 8 (i / 4) + 4 half + i % 4 of the tile.
     if constexpr (!kWide) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -514,12 +542,12 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
           s[kb][4 * g + 3] *= f.w;
         }
     }
+    if constexpr (kExtras) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x = s[kb][i] * c;
-        if constexpr (kExtras) {
+        for (int i = 0; i < 16; ++i) {
+          float x = s[kb][i] * c;
           if (capped) {
             // cap * tanh(x / cap) = cap * (1 - 2 / (e^(2 x / cap) + 1)), in base 2
             const float e = fast_exp2(x * (2.f / p.softcap));
@@ -527,9 +555,9 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
           }
           const int key = key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
           x -= slope * (float)abs(pos - key);
+          s[kb][i] = x;
         }
-        s[kb][i] = x;
-      }
+    }
     // Tiles with keys that some row of the wave does not see.
     const bool full = key0 + KT - 1 <= (p.causal ? min(pos_lo, sq.len - 1) : sq.len - 1) &&
                       (p.window_left < 0 || key0 >= pos_hi - p.window_left);
@@ -548,6 +576,7 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
     for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[0][i]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[1][i]);
+    mt *= cs;
     if (__builtin_amdgcn_ballot_w64(mt > m + kPrefillRescaleLog2) != 0) {  // wave-uniform
       const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt),
                                                        false, false);
@@ -566,8 +595,8 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[kb][i] = fast_exp2(s[kb][i] - mr);
-        l += s[kb][i];
+        s[kb][i] = fast_exp2(__builtin_fmaf(s[kb][i], cs, -mr));
+        if constexpr (!kWide) l += s[kb][i];
       }
     if constexpr (!kWide) {
 #pragma unroll
@@ -593,6 +622,9 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
         w[jj] = Prod32<TV>::pack(a, b);
         if constexpr (kSplitP)
           x[jj] = Prod32<TV>::pack(a - Elem<BF16>::lo(w[jj]), b - Elem<BF16>::hi(w[jj]));
+        // The sum of the rounded weights: the output is then a mean of V rows, and a pair
+        // takes one instruction. (8-bit rows: the weights carry vs; summed above.)
+        if constexpr (kWide) l = Prod32<T>::add_pair(w[jj], l);
       }
       pf[st] = make_uint4(w[0], w[1], w[2], w[3]);
       if constexpr (kSplitP) pl[st] = make_uint4(x[0], x[1], x[2], x[3]);
@@ -611,7 +643,7 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
           const int r = st * 16 + 8 * u + v_key;
           const int byte = (d * 32 + v_dim) * 2;
           const int at =
-              r * kRowBytes + (((byte >> 4) ^ swizzle_v(r)) << 4) + (byte & 15);
+              r * kRowBytes + (((byte >> 4) ^ swizzle_v<HD>(r)) << 4) + (byte & 15);
           typedef __attribute__((address_space(3))) s16x4v LdsVec;
           const s16x4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec *)(lds_v[buf] + at));
           const uint2 y = __builtin_bit_cast(uint2, x);
