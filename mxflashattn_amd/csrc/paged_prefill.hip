@@ -13,8 +13,6 @@ namespace {
 
 bool al(const void *ptr, uintptr_t n) { return ((uintptr_t)ptr & (n - 1)) == 0; }
 
-int rows_of(int hd) { return hd == 256 ? kPrefillRows<256> : kPrefillRows<128>; }
-
 // Fewest keys of a piece.
 constexpr int kLeastKeys = 256;
 
@@ -23,7 +21,7 @@ constexpr int kLeastKeys = 256;
 int target_of(int batch, int rows_q, int gq, int hkv, int hd, int64_t max_len, int num_cus) {
   if (max_len <= kLeastKeys) return 0;
   const int target = (2 * num_cus + hkv - 1) / hkv;
-  const int64_t tiles = ((int64_t)rows_q * gq + rows_of(hd) - 1) / rows_of(hd);
+  const int64_t tiles = ((int64_t)rows_q * gq + kPrefillRows - 1) / kPrefillRows;
   // One sequence: its tiles all span the same keys, W / target or fewer from here on.
   if (batch == 1 && tiles >= target) return 0;
   return target;
@@ -37,7 +35,7 @@ struct Layout {
 // The pieces of tiles that are cut: at most two per piece aimed at (a tile is cut into
 // ceil(span / most) < 2 span / most pieces, and most >= W / target).
 Layout layout(int target, int hkv, int hd) {
-  const size_t slots = (size_t)2 * target * hkv, rows = rows_of(hd);
+  const size_t slots = (size_t)2 * target * hkv, rows = kPrefillRows;
   Layout w;
   w.o = 0;
   w.lse = slots * rows * hd * 4;
@@ -121,7 +119,7 @@ int mxfa_package_prefill_launch(
                  : !heads_apart)
     return MXFA_EINVAL;
   if (window_left < -1 || !(softcap >= 0.f) || isinf(softcap)) return MXFA_EINVAL;
-  const int gq = q_heads / kv_heads, rows = rows_of(head_dim);
+  const int gq = q_heads / kv_heads, rows = kPrefillRows;
   const int target = target_of(batch, rows_q, gq, kv_heads, head_dim, max_len, num_cus);
   const Layout w = layout(target, kv_heads, head_dim);
   if (w.bytes && (!workspace || !al(workspace, 16) || workspace_bytes < w.bytes))

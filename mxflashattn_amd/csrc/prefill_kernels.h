@@ -38,6 +38,7 @@
 #include <stdint.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "mxfa_device.h"
 #include "mxfa_mi355x.h"
@@ -82,12 +83,19 @@ struct PrefillParams {
   int uniform;  // pages of 16 tokens or more (and rows within 32-bit offsets of each other)
 };
 
-// Waves of a workgroup, 32 rows each: eight, two per SIMD; at head dim 256, whose
-// accumulators alone are 128 registers, four with all of a SIMD's registers each.
-template <int HD>
+// Waves of a workgroup, 32 rows each. Two workgroups of four share a CU where one of eight
+// would fit: they are not in step, so one's exponentials meet the other's products, and the
+// last workgroups of a call leave less of the chip idle (six prompts of 300-1500 tokens,
+// 32q/8kv HD 128: 90.8 us against 112.6; a long chunk, before rows went straight to LDS,
+// 2661 against 2369).
 constexpr int kPrefillWaves = 4;
-template <int HD>
-constexpr int kPrefillRows = 32 * kPrefillWaves<HD>;
+constexpr int kPrefillRows = 32 * kPrefillWaves;
+// Workgroups per CU, as far as the registers of their waves (one per SIMD each) reach: the
+// accumulators are HD / 2 registers, q HD / 4.
+template <int HD, typename T, int kCache, bool kExtras>
+constexpr int kPrefillOccupancy = HD == 256 || (HD == 128 && kExtras && kCache != kCache16) ? 1
+                                  : HD == 64 && kCache == kCache16                       ? 3
+                                                                                         : 2;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4v __attribute__((ext_vector_type(4)));
@@ -164,15 +172,33 @@ __device__ __forceinline__ uint32_t lds_offset(const char *ptr) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)ptr;
 }
 
+// A pointer that is the same in every lane, as a scalar.
+__device__ __forceinline__ const char *uniform_pointer(const char *ptr) {
+  const uint64_t x = (uint64_t)ptr;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (const char *)(((uint64_t)hi << 32) | lo);
+}
+
 // 16 bytes a lane from base + off (base the same in the whole wave) to LDS at `lds` + 16 *
 // lane, with no register in between. The compiler does not see the load: the caller waits
 // for it (vmcnt) ahead of the barrier that hands the data over. (The builtin for it makes
-// the compiler wait at the next LDS read, of the other buffer.)
+// the compiler wait at the next LDS read, of the other buffer. It keeps nothing in m0.)
 __device__ __forceinline__ void load_to_lds(const char *base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(lds), "v"(off), "s"(base)
-               : "memory", "m0");
+               : "memory");
+}
+
+// f(std::integral_constant<int, I>) for I = 0 .. N-1, unrolled at compile time.
+template <typename F, int... I>
+__device__ __forceinline__ void static_unroll_impl(F &&f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_unroll(F &&f) {
+  static_unroll_impl(f, std::make_integer_sequence<int, N>{});
 }
 
 // What one sequence asks for: its query rows and keys, held to those that exist.
@@ -282,7 +308,10 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
   }
   if (tell && p.target > 0 && threadIdx.x == 0) *p.ws_total = min(slots_all, p.max_slots);
   __syncthreads();
-  return s.item;
+  // The same in every lane: scalars, and so is what follows from them.
+  const auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  return {uniform(s.item.b), uniform(s.item.tile), uniform(s.item.piece), uniform(s.item.pieces),
+          uniform(s.item.slot)};
 }
 
 // One row tile (and piece of its keys) of one kv head.
@@ -292,16 +321,18 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
 // without passing through registers (a lane loads the chunk that belongs where its 16
 // bytes land). Page ids are read a tile ahead of the loads, those a tile ahead of the math.
 template <int HD, typename T, int kCache, bool kExtras, bool kUniform>
-__global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(PrefillParams p) {
-  constexpr int kThreads = kPrefillWaves<HD> * 64;
-  constexpr int kRows = kPrefillRows<HD>;
+__global__ __launch_bounds__(kPrefillWaves * 64, (kPrefillOccupancy<HD, T, kCache, kExtras>))
+void paged_prefill_kernel(PrefillParams p) {
+  constexpr int kThreads = kPrefillWaves * 64;
+  constexpr int kRows = kPrefillRows;
   constexpr int KT = kPrefillKeys;
   constexpr int kRowBytes = HD * 2;              // of a row in LDS
   constexpr bool kWide = kCache == kCache16;
   constexpr int kLoadBytes = kWide ? HD * 2 : HD;  // of a row in the cache
   constexpr int kLoads = kLoadBytes / 16;          // its 16-byte loads
-  constexpr int kPass = kThreads / kLoads;         // rows that one load of every thread covers
-  constexpr int kPer = kPass >= KT ? 1 : KT / kPass;
+  constexpr int kWaveRows = 64 / kLoads;           // rows that one load of a wave covers
+  constexpr int kWaveKeys = KT / kPrefillWaves;    // rows that a wave stages
+  constexpr int kPer = kWaveKeys / kWaveRows;      // loads of them
   constexpr int NQ = HD / 16;                      // product steps over the head dim
   constexpr int ND = HD / 32;                      // 32-dim blocks of the output
   // An fp16 call on an 8-bit cache holds V as bf16 and P as the sum of two bf16 (16 bits
@@ -320,7 +351,8 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
   if (it.b < 0) return;
   if (it.pieces > 1 && it.slot >= p.max_slots) return;
   const PrefillSeq sq = prefill_seq<kRows>(p, it.b);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // The wave's number and what follows from it are scalars.
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int gq = p.gq;
   const int rows = sq.n * gq;  // of the sequence, per kv head
@@ -342,9 +374,13 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
   const bool live = row < rows;
   const int tok = min(row, rows - 1) / gq, head = min(row, rows - 1) % gq;
   const int pos = first_pos + tok;
-  const bool wave_live = row_w < rows;
+  // Keys that all of the wave's rows see, [all_from, all_to], and the last that any does.
   const int pos_lo = first_pos + row_w / gq;
   const int pos_hi = first_pos + min(row_w + 31, rows - 1) / gq;
+  const int all_to = p.causal ? min(pos_lo, sq.len - 1) : sq.len - 1;
+  const int all_from = p.window_left < 0 ? 0 : pos_hi - p.window_left;
+  const int any_to = row_w >= rows ? -1
+                                   : min(p.causal ? pos_hi : sq.len - 1, k_begin + j1 * KT - 1);
   const int lim = p.causal ? min(pos, sq.len - 1) : sq.len - 1;  // last key the row sees
   const int from = p.window_left >= 0 ? pos - p.window_left : 0;  // and the first
 
@@ -373,135 +409,167 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
   const bool capped = kExtras && p.softcap > 0.f;
   const float slope = kExtras && p.alibi ? p.alibi[kvh * gq + head] * kPrefillLog2e : 0.f;
 
-  // Staging: thread (row, chunk) of each pass; a wave's rows follow each other.
-  constexpr int kWaveRows = 64 / kLoads;
+  // Staging: a wave brings kWaveKeys = 16 consecutive rows (kUniform: of one page), a lane
+  // 16 bytes of every kWaveRows-th of them.
+  static_assert(kPer >= 1 && kWaveKeys == 16, "whole loads, rows of one page");
   constexpr bool kDirect = kWide && kUniform;
-  const int s_row = threadIdx.x / kLoads, s_chunk = threadIdx.x % kLoads;
-  const int w_row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kWaveRows;
+  const int l_row = lane / kLoads, l_chunk = lane % kLoads;
+  const int w_row = wave * kWaveKeys;
   const int ps_mask = (1 << p.ps_log2) - 1;
   const int last_page = (p.max_len - 1) >> p.ps_log2;
   const int32_t *bt = p.bt + (int64_t)it.b * p.bt_stride;
   const int64_t head_off = (int64_t)kvh * p.sh;
-  // Byte offsets of this lane from its wave's first row (kUniform). A pass of eight rows
-  // (head dim 256) swaps K's chunk halves every other time.
-  static_assert(!kDirect || kPass % 16 == 0 || (HD == 256 && kPass % 8 == 0), "swizzle_k");
-  const uint32_t lane_row = (uint32_t)(s_row & (kWaveRows - 1)) * (uint32_t)p.st;
-  const uint32_t k_off = lane_row + (kDirect ? (s_chunk ^ swizzle_k<HD>(s_row)) : s_chunk) * 16;
-  const uint32_t k_off_odd =
-      kPass % 16 == 0 ? k_off : lane_row + (s_chunk ^ swizzle_k<HD>(s_row + kPass)) * 16;
-  const uint32_t v_off = lane_row + (kDirect ? (s_chunk ^ swizzle_v<HD>(s_row)) : s_chunk) * 16;
+  const uint32_t st = (uint32_t)p.st;  // kUniform: below 2^24
+  // Byte offset of this lane from the first of the rows that a load covers (kUniform).
+  const uint32_t lane_off = (uint32_t)l_row * st;
   uint4 rk[kDirect ? 1 : kPer], rv[kDirect ? 1 : kPer];
-  float rks = 0.f, rvs = 0.f;  // 8-bit: the scales of the tile's key threadIdx.x
-  int pg[kPer], pg_scale = 0;  // page ids of the tile to load next
+  // K's stage j holds the keys that come 32 behind V's tile j: the second half of tile j and
+  // the first of tile j + 1.
+  constexpr int kAhead = KT / 2;
+  float rks = 0.f, rvk = 0.f, rvs = 0.f;  // 8-bit: scales of stage row `lane` (vs at K's key too)
+  // Page ids of the rows to load next: one for the wave's rows of K and of V (kUniform), else
+  // one for each of this lane's.
+  constexpr int kPages = kUniform ? 1 : kPer;
+  int pg_k[kPages], pg_v[kPages], pg_ks = 0, pg_vs = 0;
 
-  // Page ids as the table has them, of keys that may lie past the sequence: the index is
+  // As the table has them, of keys that may lie before or past the sequence: the index is
   // held to the table's row here, the id to the cache where it is used.
+  auto page_at = [&](int key) { return min(max(key, 0) >> p.ps_log2, last_page); };
   auto find_pages = [&](int j) {
     const int key0 = k_begin + j * KT;
 #pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      const int r = u * kPass + (kUniform ? w_row : s_row);
-      const int at = min((key0 + min(r, KT - 1)) >> p.ps_log2, last_page);
-      if constexpr (kUniform)
-        pg[u] = ((const __attribute__((address_space(4))) int32_t *)bt)[at];
-      else
-        pg[u] = bt[at];
+    for (int u = 0; u < kPages; ++u) {
+      const int r = w_row + (kUniform ? 0 : u * kWaveRows + l_row);
+      if constexpr (kUniform) {
+        const auto table = (const __attribute__((address_space(4))) int32_t *)bt;
+        pg_k[u] = table[page_at(key0 + kAhead + r)];
+        pg_v[u] = table[page_at(key0 + r)];
+      } else {
+        pg_k[u] = bt[page_at(key0 + kAhead + r)];
+        pg_v[u] = bt[page_at(key0 + r)];
+      }
     }
     if constexpr (!kWide) {
-      if (threadIdx.x < KT) pg_scale = bt[min((key0 + (int)threadIdx.x) >> p.ps_log2, last_page)];
+      if (wave == 0) {
+        pg_ks = bt[page_at(key0 + kAhead + lane)];
+        pg_vs = bt[page_at(key0 + lane)];
+      }
     }
   };
-  auto page_off = [&](int page) -> int64_t {
-    return (int64_t)min(max(page, 0), p.num_pages - 1) * p.sp;
+  // Offset in the cache of key's row of this head.
+  auto row_off = [&](int key, int page) -> int64_t {
+    page = min(max(page, 0), p.num_pages - 1);
+    if constexpr (kUniform)
+      return (int64_t)page * p.sp + (head_off + (uint32_t)(key & ps_mask) * (uint64_t)st);
+    return (int64_t)page * p.sp + (int64_t)(key & ps_mask) * p.st + head_off;
+  };
+  auto load_rows = [&](const char *side, int key0, const int (&pg)[kPages], auto is_k, char *lds,
+                       uint4 (&reg)[kDirect ? 1 : kPer]) {
+    if constexpr (kUniform) {
+      const char *src = uniform_pointer(side + row_off(key0 + w_row, pg[0]));
+      uint32_t at = lds_offset(lds) + w_row * kRowBytes;
+      static_unroll<kPer>([&](auto uc) {
+        constexpr int u = decltype(uc)::value;
+        // The lane whose 16 bytes land at chunk l_chunk of the LDS row loads the chunk that
+        // belongs there.
+        const int r = u * kWaveRows + l_row;  // of the wave's 16, which start a multiple of 16
+        const int from = !kDirect ? l_chunk
+                         : decltype(is_k)::value ? l_chunk ^ swizzle_k<HD>(r)
+                                                 : l_chunk ^ swizzle_v<HD>(r);
+        if constexpr (kDirect)
+          load_to_lds(src, lane_off + from * 16, at);
+        else
+          reg[u] = *reinterpret_cast<const uint4 *>(src + lane_off + from * 16);
+        src += kWaveRows * st;
+        at += kWaveRows * kRowBytes;
+      });
+    } else {
+#pragma unroll
+      for (int u = 0; u < kPer; ++u)
+        reg[u] = *reinterpret_cast<const uint4 *>(
+            side + row_off(key0 + w_row + u * kWaveRows + l_row, pg[u]) + l_chunk * 16);
+    }
+  };
+  auto load_k_scales = [&](int key0) {
+    if constexpr (!kWide) {
+      if (wave == 0) {
+        const int off = (key0 + lane) & ps_mask;
+        const int64_t page = min(max(pg_ks, 0), p.num_pages - 1);
+        rks = p.ks ? p.ks[page * p.ks_sp + (int64_t)kvh * p.ks_sh + off] : 1.f;
+        rvk = p.vs ? p.vs[page * p.vs_sp + (int64_t)kvh * p.vs_sh + off] : 1.f;
+      }
+    }
   };
   auto load_tile = [&](int j, int buf) {
     const int key0 = k_begin + j * KT;
-#pragma unroll
-    for (int u = 0; u < kPer; ++u) {
-      if constexpr (kUniform) {
-        if (kPass * kPer > KT && u * kPass + w_row >= KT) break;
-        const int64_t off = page_off(pg[u]) +
-                            (int64_t)((key0 + u * kPass + w_row) & ps_mask) * p.st + head_off;
-        if constexpr (kDirect) {
-          const uint32_t at = (u * kPass + w_row) * kRowBytes;
-          load_to_lds(p.k + off, u & 1 ? k_off_odd : k_off, lds_offset(lds_k[buf]) + at);
-          load_to_lds(p.v + off, v_off, lds_offset(lds_v[buf]) + at);
-        } else {
-          rk[u] = *reinterpret_cast<const uint4 *>(p.k + off + k_off);
-          rv[u] = *reinterpret_cast<const uint4 *>(p.v + off + v_off);
-        }
-      } else {
-        const int r = min(s_row + u * kPass, KT - 1);
-        const int64_t off = page_off(pg[u]) + (int64_t)((key0 + r) & ps_mask) * p.st + head_off +
-                            s_chunk * 16;
-        rk[u] = *reinterpret_cast<const uint4 *>(p.k + off);
-        rv[u] = *reinterpret_cast<const uint4 *>(p.v + off);
-      }
-    }
+    load_rows(p.k, key0 + kAhead, pg_k, std::true_type{}, lds_k[buf], rk);
+    load_rows(p.v, key0, pg_v, std::false_type{}, lds_v[buf], rv);
+    load_k_scales(key0 + kAhead);
     if constexpr (!kWide) {
-      if (threadIdx.x < KT) {
-        const int key = key0 + threadIdx.x;
-        const int64_t page = min(max(pg_scale, 0), p.num_pages - 1);
-        rks = p.ks ? p.ks[page * p.ks_sp + (int64_t)kvh * p.ks_sh + (key & ps_mask)] : 1.f;
-        rvs = p.vs ? p.vs[page * p.vs_sp + (int64_t)kvh * p.vs_sh + (key & ps_mask)] : 1.f;
+      if (wave == 0) {
+        const int64_t page = min(max(pg_vs, 0), p.num_pages - 1);
+        rvs = p.vs ? p.vs[page * p.vs_sp + (int64_t)kvh * p.vs_sh + ((key0 + lane) & ps_mask)]
+                   : 1.f;
       }
     }
   };
-  // The tile into LDS (kDirect: it is on its way there; this thread's loads are waited for).
-  // V rows at or past the sequence's end become zeros, whatever their memory holds; their
-  // keys are masked.
-  auto store_tile = [&](int j, int buf) {
-    const int valid = sq.len - (k_begin + j * KT);  // rows of the tile that exist
-    if constexpr (kDirect) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (valid < KT) {
-#pragma unroll
-        for (int u = 0; u < kPer; ++u) {
-          const int r = s_row + u * kPass;
-          if (r >= valid && r < KT)
-            *reinterpret_cast<uint4 *>(lds_v[buf] + r * kRowBytes + s_chunk * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-    } else {
+  // Rows from registers to LDS, an 8-bit cache's widened; zeros from row `valid` on.
+  auto store_rows = [&](const uint4 (&reg)[kDirect ? 1 : kPer], char *lds, auto type, auto is_k,
+                        int valid) {
+    using TR = decltype(type);
+    if constexpr (!kDirect) {
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
-        const int r = s_row + u * kPass;
-        const uint4 wk = rk[u];
-        const bool there = r < valid;
-        const uint4 wv = make_uint4(there ? rv[u].x : 0u, there ? rv[u].y : 0u,
-                                    there ? rv[u].z : 0u, there ? rv[u].w : 0u);
-        const int sk = swizzle_k<HD>(r), sv = swizzle_v<HD>(r);
-        if (r < KT) {
-          char *dk = lds_k[buf] + r * kRowBytes, *dv = lds_v[buf] + r * kRowBytes;
-          if constexpr (kWide) {
-            *reinterpret_cast<uint4 *>(dk + (s_chunk ^ sk) * 16) = wk;
-            *reinterpret_cast<uint4 *>(dv + (s_chunk ^ sv) * 16) = wv;
-          } else {
-            const uint2 k0 = widen_codes<T, kCache>(wk.x), k1 = widen_codes<T, kCache>(wk.y);
-            const uint2 k2 = widen_codes<T, kCache>(wk.z), k3 = widen_codes<T, kCache>(wk.w);
-            const uint2 v0 = widen_codes<TV, kCache>(wv.x), v1 = widen_codes<TV, kCache>(wv.y);
-            const uint2 v2 = widen_codes<TV, kCache>(wv.z), v3 = widen_codes<TV, kCache>(wv.w);
-            *reinterpret_cast<uint4 *>(dk + ((2 * s_chunk) ^ sk) * 16) =
-                make_uint4(k0.x, k0.y, k1.x, k1.y);
-            *reinterpret_cast<uint4 *>(dk + ((2 * s_chunk + 1) ^ sk) * 16) =
-                make_uint4(k2.x, k2.y, k3.x, k3.y);
-            *reinterpret_cast<uint4 *>(dv + ((2 * s_chunk) ^ sv) * 16) =
-                make_uint4(v0.x, v0.y, v1.x, v1.y);
-            *reinterpret_cast<uint4 *>(dv + ((2 * s_chunk + 1) ^ sv) * 16) =
-                make_uint4(v2.x, v2.y, v3.x, v3.y);
-          }
+        const int r = w_row + u * kWaveRows + l_row;
+        uint4 w = reg[u];
+        if constexpr (!decltype(is_k)::value) {
+          const bool there = r < valid;
+          w = make_uint4(there ? w.x : 0u, there ? w.y : 0u, there ? w.z : 0u, there ? w.w : 0u);
+        }
+        const int sw = decltype(is_k)::value ? swizzle_k<HD>(r) : swizzle_v<HD>(r);
+        char *dst = lds + r * kRowBytes;
+        if constexpr (kWide) {
+          *reinterpret_cast<uint4 *>(dst + (l_chunk ^ sw) * 16) = w;
+        } else {
+          const uint2 a = widen_codes<TR, kCache>(w.x), b = widen_codes<TR, kCache>(w.y);
+          const uint2 c = widen_codes<TR, kCache>(w.z), d = widen_codes<TR, kCache>(w.w);
+          *reinterpret_cast<uint4 *>(dst + ((2 * l_chunk) ^ sw) * 16) =
+              make_uint4(a.x, a.y, b.x, b.y);
+          *reinterpret_cast<uint4 *>(dst + ((2 * l_chunk + 1) ^ sw) * 16) =
+              make_uint4(c.x, c.y, d.x, d.y);
         }
       }
+    }
+  };
+  auto store_k = [&](int buf) {
+    store_rows(rk, lds_k[buf], T{}, std::true_type{}, KT);
+    // A V row without a scale (NaN: it held an infinity or a NaN) takes its key's score along
+    // instead, so that it reaches the rows that see the key and no other (a weight of zero
+    // times NaN would).
+    if constexpr (!kWide) {
+      if (wave == 0) lds_ks[buf][lane] = fabsf(rvk) < INFINITY ? rks : __builtin_nanf("");
+    }
+  };
+  // The loaded rows into LDS (kDirect: they are on their way there; this wave's are waited
+  // for). V rows at or past the sequence's end become zeros, whatever their memory holds;
+  // their keys are masked.
+  auto store_tile = [&](int j, int buf) {
+    const int valid = sq.len - (k_begin + j * KT);  // V rows of the tile that exist
+    if constexpr (kDirect) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (valid < KT) {  // once a sequence
+        int r = w_row + l_row;
+        asm volatile("" : "+v"(r));  // nothing of this is worth registers in the loop
+        for (int u = 0; u < kPer; ++u, r += kWaveRows)
+          if (r >= valid)
+            *reinterpret_cast<uint4 *>(lds_v[buf] + r * kRowBytes + l_chunk * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else {
+      store_k(buf);
+      store_rows(rv, lds_v[buf], TV{}, std::false_type{}, valid);
       if constexpr (!kWide) {
-        if (threadIdx.x < KT) {
-          // A V row without a scale (NaN: it held an infinity or a NaN) takes its key's score
-          // along instead, so that it reaches the rows that see the key and no other (a
-          // weight of zero times NaN would).
-          const bool whole = fabsf(rvs) < INFINITY;
-          lds_ks[buf][threadIdx.x] = whole ? rks : __builtin_nanf("");
-          lds_vs[buf][threadIdx.x] = whole && (int)threadIdx.x < valid ? rvs : 0.f;
-        }
+        if (wave == 0) lds_vs[buf][lane] = fabsf(rvs) < INFINITY && lane < valid ? rvs : 0.f;
       }
     }
   };
@@ -513,72 +581,66 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
 
-  auto compute = [&](int buf, int key0) {
-    f32x16 s[2];
+  // K operands of the 32 keys in rows r0.. of buffer buf.
+  uint4 kf[NQ];
+  auto read_k = [&](int buf, int r0) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
-      const int r = kb * 32 + col;
-      const char *base = lds_k[buf] + r * kRowBytes;
-#pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        const uint4 a = *reinterpret_cast<const uint4 *>(
-            base + (((2 * i + half) ^ swizzle_k<HD>(r)) * 16));
-        s[kb] = Prod32<T>::run(a, qf[i], s[kb]);
-      }
-    }
-    // Scores: keys kb * 32 + 8 (i / 4) + 4 half + i % 4 of the tile.
+    for (int i = 0; i < NQ; ++i)
+      kf[i] = *reinterpret_cast<const uint4 *>(
+          lds_k[buf] + (r0 + col) * kRowBytes + (((2 * i + half) ^ swizzle_k<HD>(col)) * 16));
+  };
+  // The scales of an 8-bit cache's rows: scores keys 8 (i / 4) + 4 half + i % 4 of the 32.
+  auto scale_scores = [&](int buf, int r0, f32x16 &s) {
     if constexpr (!kWide) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 f =
-              *reinterpret_cast<const float4 *>(&lds_ks[buf][kb * 32 + 8 * g + 4 * half]);
-          s[kb][4 * g] *= f.x;
-          s[kb][4 * g + 1] *= f.y;
-          s[kb][4 * g + 2] *= f.z;
-          s[kb][4 * g + 3] *= f.w;
-        }
+      for (int g = 0; g < 4; ++g) {
+        const float4 f = *reinterpret_cast<const float4 *>(&lds_ks[buf][r0 + 8 * g + 4 * half]);
+        s[4 * g] *= f.x;
+        s[4 * g + 1] *= f.y;
+        s[4 * g + 2] *= f.z;
+        s[4 * g + 3] *= f.w;
+      }
     }
+  };
+  const auto largest = [&](const f32x16 &s) {
+    float x = fmaxf(s[0], s[1]);
+#pragma unroll
+    for (int i = 2; i < 16; ++i) x = fmaxf(x, s[i]);
+    return x;
+  };
+  // Options and masks; top: the lane's largest score.
+  auto limit = [&](int key0, f32x16 &s, float &top) {
     if constexpr (kExtras) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float x = s[kb][i] * c;
-          if (capped) {
-            // cap * tanh(x / cap) = cap * (1 - 2 / (e^(2 x / cap) + 1)), in base 2
-            const float e = fast_exp2(x * (2.f / p.softcap));
-            x = p.softcap * kPrefillLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
-          }
-          const int key = key0 + kb * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-          x -= slope * (float)abs(pos - key);
-          s[kb][i] = x;
+      for (int i = 0; i < 16; ++i) {
+        float x = s[i] * c;
+        if (capped) {
+          // cap * tanh(x / cap) = cap * (1 - 2 / (e^(2 x / cap) + 1)), in base 2
+          const float e = fast_exp2(x * (2.f / p.softcap));
+          x = p.softcap * kPrefillLog2e * (1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f));
         }
+        const int key = key0 + 8 * (i >> 2) + 4 * half + (i & 3);
+        x -= slope * (float)abs(pos - key);
+        s[i] = x;
+      }
+      top = largest(s);
     }
-    // Tiles with keys that some row of the wave does not see.
-    const bool full = key0 + KT - 1 <= (p.causal ? min(pos_lo, sq.len - 1) : sq.len - 1) &&
-                      (p.window_left < 0 || key0 >= pos_hi - p.window_left);
-    if (!full) {
+    // Keys that some row of the wave does not see.
+    if (key0 + 31 > all_to || key0 < all_from) {
       const int hi = lim - key0 - 4 * half, lo = from - key0 - 4 * half;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = kb * 32 + 8 * (i >> 2) + (i & 3);
-          s[kb][i] = (k <= hi && k >= lo) ? s[kb][i] : -INFINITY;
-        }
+      for (int i = 0; i < 16; ++i) {
+        const int k = 8 * (i >> 2) + (i & 3);
+        s[i] = (k <= hi && k >= lo) ? s[i] : -INFINITY;
+      }
+      top = largest(s);
     }
-    float mt = s[0][0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mt = fmaxf(mt, s[0][i]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[1][i]);
-    mt *= cs;
-    if (__builtin_amdgcn_ballot_w64(mt > m + kPrefillRescaleLog2) != 0) {  // wave-uniform
-      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mt), __float_as_uint(mt),
+  };
+  // Moves the reference where a score passed it by more than kPrefillRescaleLog2.
+  auto refer = [&](float top) {
+    top *= cs;
+    if (__builtin_amdgcn_ballot_w64(top > m + kPrefillRescaleLog2) != 0) {  // wave-uniform
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
                                                        false, false);
       const float mm = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
       const float mn = mm > m + kPrefillRescaleLog2 ? mm : m;
@@ -590,96 +652,151 @@ __global__ __launch_bounds__(kPrefillWaves<HD> * 64) void paged_prefill_kernel(P
         for (int i = 0; i < 16; ++i) o[d][i] *= f;
       m = mn;
     }
-    const float mr = m == -INFINITY ? 0.f : m;  // no key seen yet: the scores here are -inf too
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[kb][i] = fast_exp2(__builtin_fmaf(s[kb][i], cs, -mr));
-        if constexpr (!kWide) l += s[kb][i];
-      }
+  };
+  // Weights of 32 keys (V rows r0.. of buffer buf), rounded once (the 16-bit products take no
+  // more): eight keys per operand register set. Score i's part of it: pairs are packed and
+  // summed as they come.
+  uint32_t pf[8], pl[kSplitP ? 8 : 1];
+  float mr;  // the reference; 0 where no key is seen yet (the scores are -inf then)
+  float4 vsc[kWide ? 1 : 4];
+  auto weigh_start = [&](int buf, int r0) {
+    mr = m == -INFINITY ? 0.f : m;
     if constexpr (!kWide) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 f =
-              *reinterpret_cast<const float4 *>(&lds_vs[buf][kb * 32 + 8 * g + 4 * half]);
-          s[kb][4 * g] *= f.x;
-          s[kb][4 * g + 1] *= f.y;
-          s[kb][4 * g + 2] *= f.z;
-          s[kb][4 * g + 3] *= f.w;
-        }
-    }
-    // P rounded once (the 16-bit products take no more), eight keys per operand register set.
-    uint4 pf[4], pl[kSplitP ? 4 : 1];
-#pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      uint32_t w[4], x[4];
-#pragma unroll
-      for (int jj = 0; jj < 4; ++jj) {
-        const float a = s[st >> 1][8 * (st & 1) + 2 * jj], b = s[st >> 1][8 * (st & 1) + 2 * jj + 1];
-        w[jj] = Prod32<TV>::pack(a, b);
-        if constexpr (kSplitP)
-          x[jj] = Prod32<TV>::pack(a - Elem<BF16>::lo(w[jj]), b - Elem<BF16>::hi(w[jj]));
-        // The sum of the rounded weights: the output is then a mean of V rows, and a pair
-        // takes one instruction. (8-bit rows: the weights carry vs; summed above.)
-        if constexpr (kWide) l = Prod32<T>::add_pair(w[jj], l);
-      }
-      pf[st] = make_uint4(w[0], w[1], w[2], w[3]);
-      if constexpr (kSplitP) pl[st] = make_uint4(x[0], x[1], x[2], x[3]);
-    }
-    // V^T operand: lane l reads dims 16 ((l / 16) % 2) + 4 (l % 4) .. of key
-    // 4 (l / 32) + (l / 4) % 4 and receives dim l % 32 of four keys.
-    const int v_key = 4 * half + ((lane >> 2) & 3);
-    const int v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);  // within the 32-dim block
-#pragma unroll
-    for (int st = 0; st < 4; ++st) {
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        uint32_t w[4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int r = st * 16 + 8 * u + v_key;
-          const int byte = (d * 32 + v_dim) * 2;
-          const int at =
-              r * kRowBytes + (((byte >> 4) ^ swizzle_v<HD>(r)) << 4) + (byte & 15);
-          typedef __attribute__((address_space(3))) s16x4v LdsVec;
-          const s16x4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec *)(lds_v[buf] + at));
-          const uint2 y = __builtin_bit_cast(uint2, x);
-          w[2 * u] = y.x;
-          w[2 * u + 1] = y.y;
-        }
-        const uint4 a = make_uint4(w[0], w[1], w[2], w[3]);
-        o[d] = Prod32<TV>::run(a, pf[st], o[d]);
-        if constexpr (kSplitP) o[d] = Prod32<TV>::run(a, pl[st], o[d]);
-      }
+      for (int g = 0; g < 4; ++g)
+        vsc[g] = *reinterpret_cast<const float4 *>(&lds_vs[buf][r0 + 8 * g + 4 * half]);
     }
   };
-
+  auto weigh = [&](auto ic, f32x16 &s) {
+    constexpr int i = decltype(ic)::value;
+    s[i] = fast_exp2(__builtin_fmaf(s[i], cs, -mr));
+    if constexpr (!kWide) {
+      l += s[i];
+      s[i] *= (i & 3) == 0 ? vsc[i >> 2].x
+              : (i & 3) == 1 ? vsc[i >> 2].y
+              : (i & 3) == 2 ? vsc[i >> 2].z
+                             : vsc[i >> 2].w;
+    }
+    if constexpr (i & 1) {
+      pf[i >> 1] = Prod32<TV>::pack(s[i - 1], s[i]);
+      if constexpr (kSplitP)
+        pl[i >> 1] = Prod32<TV>::pack(s[i - 1] - Elem<BF16>::lo(pf[i >> 1]),
+                                      s[i] - Elem<BF16>::hi(pf[i >> 1]));
+      // The sum of the rounded weights: the output is then a mean of V rows, and a pair
+      // takes one instruction. (8-bit rows: the weights carry vs; summed above.)
+      if constexpr (kWide) l = Prod32<T>::add_pair(pf[i >> 1], l);
+    }
+  };
+  // V^T operand: lane l reads dims 16 ((l / 16) % 2) + 4 (l % 4) .. of key
+  // 4 (l / 32) + (l / 4) % 4 and receives dim l % 32 of four keys.
+  const int v_key = 4 * half + ((lane >> 2) & 3);
+  const int v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);  // within the 32-dim block
+  auto read_v = [&](int buf, int r0, int d) {
+    uint32_t w[4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int byte = (d * 32 + v_dim) * 2;
+      const int at = (r0 + 8 * u + v_key) * kRowBytes +
+                     (((byte >> 4) ^ swizzle_v<HD>(v_key)) << 4) + (byte & 15);
+      typedef __attribute__((address_space(3))) s16x4v LdsVec;
+      const s16x4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec *)(lds_v[buf] + at));
+      const uint2 y = __builtin_bit_cast(uint2, x);
+      w[2 * u] = y.x;
+      w[2 * u + 1] = y.y;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  // The loop runs the scores of 32 keys ahead of their weights: the next keys' products fill
+  // the matrix unit while these keys' exponentials go through the VALU, a few after each
+  // product. The order is written out (sched_barrier): left to itself the compiler issues
+  // the products in a row, and a wave issues in order.
+  float top = -INFINITY;
+  auto first_scores = [&](int buf, int r0, f32x16 &s) {
+    read_k(buf, r0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) s = Prod32<T>::run(kf[i], qf[i], s);
+    scale_scores(buf, r0, s);
+    if constexpr (!kExtras) top = largest(s);
+  };
+  // The weights of cur's keys and their part of the output, and nxt's scores.
+  auto advance = [&](int buf, int r0, f32x16 &cur, f32x16 &nxt) {
+    read_k(buf, r0);
+    weigh_start(buf, r0);
+    uint4 vf[ND];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) nxt[i] = 0.f;
+    static_unroll<NQ>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      nxt = Prod32<T>::run(kf[i], qf[i], nxt);
+      static_unroll<16 / NQ>([&](auto jc) {
+        weigh(std::integral_constant<int, i * (16 / NQ) + decltype(jc)::value>{}, cur);
+      });
+      if constexpr (i >= NQ / 2) {  // the first V operands, in the second half's shadow
+        static_unroll<2 * ND / NQ>([&](auto jc) {
+          constexpr int d = (i - NQ / 2) * (2 * ND / NQ) + decltype(jc)::value;
+          vf[d] = read_v(buf, r0, d);
+        });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    uint4 vn[ND];
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const uint4 w = make_uint4(pf[4 * st], pf[4 * st + 1], pf[4 * st + 2], pf[4 * st + 3]);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const uint4 a = st ? vn[d] : vf[d];
+        o[d] = Prod32<TV>::run(a, w, o[d]);
+        if constexpr (kSplitP)
+          o[d] = Prod32<TV>::run(
+              a, make_uint4(pl[4 * st], pl[4 * st + 1], pl[4 * st + 2], pl[4 * st + 3]), o[d]);
+        if (st == 0) vn[d] = read_v(buf, r0 + 16, d);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (st == 0) scale_scores(buf, r0, nxt);
+    }
+    if constexpr (!kExtras) top = largest(nxt);
+  };
+  auto step = [&](int key0, int buf, int r0, f32x16 &cur, f32x16 &nxt) {
+    if (key0 <= any_to) {  // some row of the wave sees some of the 32 keys
+      limit(key0, cur, top);
+      refer(top);
+      advance(buf, r0, cur, nxt);  // (past the last keys, products that nobody looks at)
+    }
+  };
   if (j0 < j1) {
+    f32x16 sa, sb;
+    // K's stage before the first holds the first 32 keys.
+    find_pages(j0 - 1);
+    load_rows(p.k, k_begin + j0 * KT - kAhead, pg_k, std::true_type{}, lds_k[1], rk);
+    load_k_scales(k_begin + j0 * KT - kAhead);
     find_pages(j0);
+    if constexpr (!kDirect) store_k(1);
     load_tile(j0, 0);
     find_pages(j0 + 1);
-  }
-  for (int j = j0; j < j1; ++j) {
-    const int buf = (j - j0) & 1;
-    // One barrier a tile: past it the tile's rows are there, and every wave is done with
-    // the other buffer, which the next tile's loads then fill.
-    store_tile(j, buf);
-    if (!kDirect && j + 1 < j1) {
-      load_tile(j + 1, buf ^ 1);
-      find_pages(j + 2);
-    }
+    if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (kDirect && j + 1 < j1) {
-      load_tile(j + 1, buf ^ 1);
-      find_pages(j + 2);
+    first_scores(1, kAhead, sa);
+    for (int j = j0; j < j1; ++j) {
+      const int buf = (j - j0) & 1, key0 = k_begin + j * KT;
+      // One barrier a tile: past it V of tile j and K 32 keys on are in LDS, and every wave is
+      // done with the other buffers, which the next loads fill.
+      store_tile(j, buf);
+      if (!kDirect && j + 1 < j1) {
+        load_tile(j + 1, buf ^ 1);
+        find_pages(j + 2);
+      }
+      __syncthreads();
+      if (kDirect && j + 1 < j1) {
+        load_tile(j + 1, buf ^ 1);
+        find_pages(j + 2);
+      }
+      step(key0, buf, 0, sa, sb);
+      step(key0 + 32, buf, 32, sb, sa);
     }
-    const int key0 = k_begin + j * KT;
-    const bool seen = wave_live && key0 <= (p.causal ? pos_hi : sq.len - 1) &&
-                      (p.window_left < 0 || key0 + KT - 1 >= pos_lo - p.window_left);
-    if (seen) compute(buf, key0);
   }
 
   const auto lw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false,
@@ -725,7 +842,7 @@ constexpr int kPrefillJoinParts = 4;
 
 template <int HD, typename T>
 __global__ __launch_bounds__(kPrefillJoinThreads) void paged_prefill_join_kernel(PrefillParams p) {
-  constexpr int kRows = kPrefillRows<HD>;
+  constexpr int kRows = kPrefillRows;
   constexpr int kJoinRows = kPrefillJoinThreads / (HD / 4);
   const int at = blockIdx.x;  // slot * hkv + kv head
   const int slot = at / p.hkv, kvh = at - slot * p.hkv;
@@ -769,7 +886,7 @@ __global__ __launch_bounds__(kPrefillJoinThreads) void paged_prefill_join_kernel
 // Launches of one head dim (prefill_hd*.hip).
 template <int HD, typename T, int kCache>
 int launch_prefill_t(const PrefillParams &p, int items, hipStream_t st) {
-  const dim3 grid((unsigned)(items * p.hkv)), block(kPrefillWaves<HD> * 64);
+  const dim3 grid((unsigned)(items * p.hkv)), block(kPrefillWaves * 64);
   const bool extras = p.softcap > 0.f || p.alibi;
   const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, st, p); };
   if (p.uniform)
