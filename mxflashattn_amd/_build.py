@@ -107,7 +107,7 @@ _REMARK = re.compile(r"remark:\s+(Function Name|VGPRs Spill|ScratchSize \[bytes/
 # (The prefill's tiles: two buffers of K and of V, 64 rows of up to 512 bytes, their
 # scales, and its work search.)
 STATIC_LDS_LIMITS = {"split_combine_kernel": 256 * 6 * 4,
-                     "paged_prefill_kernel": 4 * 64 * 512 + 2048}
+                     "paged_prefill_kernel": 4 * 64 * 512 + 4096}
 STATIC_LDS_DEFAULT = 64
 
 

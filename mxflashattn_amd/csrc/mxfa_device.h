@@ -1,5 +1,5 @@
 // Device helpers shared by the gfx950 kernels: element types (exact widening
-// of 16-bit halves, fp32 -> fp16/bf16 rounding), the DPP row broadcast,
+// of 16-bit halves, fp32 -> fp16/bf16 rounding), the DPP row broadcast and wave scan,
 // nontemporal loads and raw buffer descriptors.
 #pragma once
 
@@ -57,6 +57,20 @@ constexpr int kDppRowBcast31 = 0x143;
 // takes lane i^1, then lane i^2).
 constexpr int kDppQuadSwap1 = 0xB1;
 constexpr int kDppQuadSwap2 = 0x4E;
+
+// Inclusive prefix sum over the 64 lanes of a wave with DPP moves only (no
+// LDS permutes): a Hillis-Steele scan inside each 16-lane row (row_shr 1, 2,
+// 4, 8), then the row totals carried across rows (row_bcast:15 into rows 1
+// and 3, row_bcast:31 into rows 2 and 3). Lanes a move leaves unwritten add 0.
+__device__ __forceinline__ int wave_scan_incl(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 1, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 2, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 4, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 8, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowBcast15, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, kDppRowBcast31, 0xc, 0xf, false);
+  return x;
+}
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

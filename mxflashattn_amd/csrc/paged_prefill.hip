@@ -171,7 +171,9 @@ int mxfa_package_prefill_launch(
   p.target = target;
   p.least = kLeastKeys;
   p.max_slots = 2 * target;
-  p.uniform = page_size >= 16 && cache_stride_token * esz < (int64_t)1 << 24;
+  p.uniform = page_size >= 16 && cache_stride_page * esz < (int64_t)1 << 32 &&
+              cache_stride_token * esz < (int64_t)1 << 24 &&
+              (int64_t)page_size * cache_stride_token * esz < (int64_t)1 << 32;
   char *ws = (char *)workspace;
   if (target) {
     p.ws_o = (float *)(ws + w.o);

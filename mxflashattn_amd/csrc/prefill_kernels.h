@@ -43,6 +43,9 @@
 #include "mxfa_device.h"
 #include "mxfa_mi355x.h"
 
+// A kernel's parts are lambdas; none may become a call.
+#define MXFA_INLINE __attribute__((always_inline))
+
 namespace mxfa {
 
 constexpr int kPrefillKeys = 64;        // keys of a tile
@@ -80,7 +83,7 @@ struct PrefillParams {
   int4 *ws_desc;         // [slot][kv head]: pieces (0 but for a tile's first), batch, tile
   int *ws_total;         // slots in use
   int max_slots;
-  int uniform;  // pages of 16 tokens or more (and rows within 32-bit offsets of each other)
+  int uniform;  // pages of 16 tokens or more, strides that 32-bit offsets reach over
 };
 
 // Waves of a workgroup, 32 rows each. Two workgroups of four share a CU where one of eight
@@ -92,10 +95,11 @@ constexpr int kPrefillWaves = 4;
 constexpr int kPrefillRows = 32 * kPrefillWaves;
 // Workgroups per CU, as far as the registers of their waves (one per SIMD each) reach: the
 // accumulators are HD / 2 registers, q HD / 4.
-template <int HD, typename T, int kCache, bool kExtras>
-constexpr int kPrefillOccupancy = HD == 256 || (HD == 128 && kExtras && kCache != kCache16) ? 1
-                                  : HD == 64 && kCache == kCache16                       ? 3
-                                                                                         : 2;
+template <int HD, typename T, int kCache, bool kExtras, bool kUniform>
+constexpr int kPrefillOccupancy =
+    HD == 256 || (HD == 128 && kExtras && (kCache != kCache16 || !kUniform)) ? 1
+    : HD == 64 && kCache == kCache16 && !kExtras                             ? 3
+                                                                             : 2;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4v __attribute__((ext_vector_type(4)));
@@ -204,77 +208,128 @@ __device__ __forceinline__ void static_unroll(F &&f) {
 // What one sequence asks for: its query rows and keys, held to those that exist.
 struct PrefillSeq {
   int start, n, len, tiles, span;
+  bool few;  // at most 32 rows in a call whose tiles may be cut: all waves on one row tile
 };
 
-template <int kRows>
 __device__ __forceinline__ PrefillSeq prefill_seq(const PrefillParams &p, int b) {
   PrefillSeq s;
   s.start = min(max(p.cu[b], 0), p.rows_q);
   const int end = min(max(p.cu[b + 1], s.start), p.rows_q);
   s.n = end - s.start;
   s.len = min(max(p.seqlens[b], 0), p.max_len);
-  s.tiles = (int)(((int64_t)s.n * p.gq + kRows - 1) / kRows);
+  const int64_t rows = (int64_t)s.n * p.gq;
+  s.few = p.target > 0 && rows <= 32;
+  s.tiles = (int)((rows + kPrefillRows - 1) / kPrefillRows);
   // Keys that one row tile spans, at most: with a window its tokens' windows together.
-  s.span = p.window_left < 0
-               ? s.len
-               : (int)min((int64_t)s.len, (int64_t)p.window_left + kRows / p.gq + 1 + kPrefillKeys);
+  s.span = p.window_left < 0 ? s.len
+                             : (int)min((int64_t)s.len, (int64_t)p.window_left +
+                                                            kPrefillRows / p.gq + 1 + kPrefillKeys);
   return s;
+}
+
+// What a key of a row tile costs: four waves on their own keys take half of a tile's time.
+__device__ __forceinline__ int prefill_cost(const PrefillSeq &q) {
+  return q.few ? (q.span + 1) / 2 : q.span;
+}
+__device__ __forceinline__ int prefill_pieces(const PrefillSeq &q, int most) {
+  const int cost = prefill_cost(q);
+  return cost > most ? (cost + most - 1) / most : 1;
+}
+// Keys (at their cost) of a piece: W / target, a little more so that 32-bit sums of W keep
+// the pieces of cut tiles within 2 * target.
+__device__ __forceinline__ int prefill_most(const PrefillParams &p, float work) {
+  if (p.target <= 0) return 0x7fffffff;
+  return max(p.least, (int)fminf(work * 1.001f / (float)p.target + 1.f, 1e9f));
 }
 
 struct PrefillItem {
   int b, tile, piece, pieces, slot;
 };
 
-template <int kThreads>
 struct PrefillScan {
-  int64_t work[kThreads / 64];
-  int items[kThreads / 64], slots[kThreads / 64];
+  float work[kPrefillWaves];
+  int items[kPrefillWaves], slots[kPrefillWaves];
   PrefillItem item;
 };
 
-// The row tile and piece of item `index`, in LDS for the whole workgroup; b = -1 past the
-// last. Tiles of a sequence in falling order: with the causal mask the later ones see more
-// keys, and the longest work goes out first.
-template <int kRows, int kThreads>
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
+// The row tile and piece of item `index`; b = -1 past the last.
+//
+// Up to 64 sequences (one a lane, every wave for itself): the last tile of every sequence,
+// then the last but one of every sequence that has it, and so on. With the causal mask a
+// sequence's later tiles see more keys, so the longest work goes out first and the end of
+// the call is made of short pieces.
+// More: sequence by sequence, in falling order too, through a scan in LDS.
 __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int index,
-                                                    PrefillScan<kThreads> &s, bool tell) {
-  constexpr int kWaves = kThreads / 64;
+                                                    PrefillScan &s, bool tell) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int per = (p.batch + kThreads - 1) / kThreads;
+  if (p.batch <= 64) {
+    const PrefillSeq q = prefill_seq(p, min(lane, p.batch - 1));
+    const int tiles = lane < p.batch ? q.tiles : 0;
+    const int most =
+        p.target > 0 ? prefill_most(p, wave_sum((float)tiles * (float)prefill_cost(q))) : 0x7fffffff;
+    const int pieces = prefill_pieces(q, most);
+    const auto total = [](int x) { return __builtin_amdgcn_readlane(wave_scan_incl(x), 63); };
+    const int cut = pieces > 1 ? tiles * pieces : 0;
+    const int slots = wave_scan_incl(cut);
+    if (tell && p.target > 0 && threadIdx.x == 0)
+      *p.ws_total = min(__builtin_amdgcn_readlane(slots, 63), p.max_slots);
+    // The round: the largest d whose items of earlier rounds are at most `index`.
+    int lo = 0, before = 0;
+    int hi = tiles;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) hi = max(hi, __shfl_xor(hi, d));
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    if (index >= total(tiles * pieces)) return {-1, 0, 0, 1, 0};
+    while (hi - lo > 1) {  // items before round lo <= index < items before round hi
+      const int mid = lo + ((hi - lo) >> 1);
+      const int items = total(pieces * min(tiles, mid));
+      if (items <= index) {
+        lo = mid;
+        before = items;
+      } else {
+        hi = mid;
+      }
+    }
+    const int here = tiles > lo ? pieces : 0;
+    const int upto = wave_scan_incl(here);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(upto > index - before);
+    const int b = past ? __builtin_ctzll(past) : 0;
+    const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
+    const int piece = index - before - (of(upto) - of(here));
+    return {b, of(tiles) - 1 - lo, piece, of(pieces),
+            of(slots) - of(cut) + lo * of(pieces) + piece};
+  }
+  const int per = (p.batch + kPrefillWaves * 64 - 1) / (kPrefillWaves * 64);
   const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
   int most = 0x7fffffff;
   if (p.target > 0) {
-    int64_t work = 0;
+    float work = 0.f;
     for (int b = b0; b < b1; ++b) {
-      const PrefillSeq q = prefill_seq<kRows>(p, b);
-      work += (int64_t)q.tiles * q.span;
+      const PrefillSeq q = prefill_seq(p, b);
+      work += (float)q.tiles * (float)prefill_cost(q);
     }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) work += __shfl_xor(work, d);
+    work = wave_sum(work);
     if (lane == 0) s.work[wave] = work;
     __syncthreads();
-    work = 0;
+    work = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) work += s.work[w];
-    const int64_t each = (work + p.target - 1) / p.target;
-    most = (int)min(max(each, (int64_t)p.least), (int64_t)0x7fffffff);
+    for (int w = 0; w < kPrefillWaves; ++w) work += s.work[w];
+    most = prefill_most(p, work);
   }
   int items = 0, slots = 0;
   for (int b = b0; b < b1; ++b) {
-    const PrefillSeq q = prefill_seq<kRows>(p, b);
-    const int pieces = q.span > most ? (q.span + most - 1) / most : 1;
+    const PrefillSeq q = prefill_seq(p, b);
+    const int pieces = prefill_pieces(q, most);
     items += q.tiles * pieces;
     slots += pieces > 1 ? q.tiles * pieces : 0;
   }
-  int items_in = items, slots_in = slots;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int a = __shfl_up(items_in, d), c = __shfl_up(slots_in, d);
-    if (lane >= d) {
-      items_in += a;
-      slots_in += c;
-    }
-  }
+  const int items_in = wave_scan_incl(items), slots_in = wave_scan_incl(slots);
   if (lane == 63) {
     s.items[wave] = items_in;
     s.slots[wave] = slots_in;
@@ -283,15 +338,15 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
   __syncthreads();
   int items_at = items_in - items, slots_at = slots_in - slots, slots_all = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < kPrefillWaves; ++w) {
     items_at += w < wave ? s.items[w] : 0;
     slots_at += w < wave ? s.slots[w] : 0;
     slots_all += s.slots[w];
   }
   if (index >= items_at && index < items_at + items) {
     for (int b = b0; b < b1; ++b) {
-      const PrefillSeq q = prefill_seq<kRows>(p, b);
-      const int pieces = q.span > most ? (q.span + most - 1) / most : 1;
+      const PrefillSeq q = prefill_seq(p, b);
+      const int pieces = prefill_pieces(q, most);
       const int here = q.tiles * pieces;
       if (index < items_at + here) {
         const int local = index - items_at;
@@ -321,9 +376,8 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
 // without passing through registers (a lane loads the chunk that belongs where its 16
 // bytes land). Page ids are read a tile ahead of the loads, those a tile ahead of the math.
 template <int HD, typename T, int kCache, bool kExtras, bool kUniform>
-__global__ __launch_bounds__(kPrefillWaves * 64, (kPrefillOccupancy<HD, T, kCache, kExtras>))
+__global__ __launch_bounds__(kPrefillWaves * 64, (kPrefillOccupancy<HD, T, kCache, kExtras, kUniform>))
 void paged_prefill_kernel(PrefillParams p) {
-  constexpr int kThreads = kPrefillWaves * 64;
   constexpr int kRows = kPrefillRows;
   constexpr int KT = kPrefillKeys;
   constexpr int kRowBytes = HD * 2;              // of a row in LDS
@@ -343,14 +397,14 @@ void paged_prefill_kernel(PrefillParams p) {
   __shared__ __align__(16) char lds_k[2][KT * kRowBytes];
   __shared__ __align__(16) char lds_v[2][KT * kRowBytes];
   __shared__ __align__(16) float lds_ks[kWide ? 1 : 2][KT], lds_vs[kWide ? 1 : 2][KT];
-  __shared__ PrefillScan<kThreads> scan;
+  __shared__ PrefillScan scan;
+  __shared__ float few_m[kPrefillWaves][32], few_l[kPrefillWaves][32];
 
   const int kvh = blockIdx.x % p.hkv;
-  const PrefillItem it =
-      prefill_find<kRows, kThreads>(p, blockIdx.x / p.hkv, scan, blockIdx.x == 0);
+  const PrefillItem it = prefill_find(p, blockIdx.x / p.hkv, scan, blockIdx.x == 0);
   if (it.b < 0) return;
   if (it.pieces > 1 && it.slot >= p.max_slots) return;
-  const PrefillSeq sq = prefill_seq<kRows>(p, it.b);
+  const PrefillSeq sq = prefill_seq(p, it.b);
   // The wave's number and what follows from it are scalars.
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
@@ -369,7 +423,7 @@ void paged_prefill_kernel(PrefillParams p) {
   const int j1 = (int)((int64_t)all * (it.piece + 1) / it.pieces);
 
   // This lane's row, and the wave's rows.
-  const int row_w = it.tile * kRows + wave * 32;
+  const int row_w = sq.few ? 0 : it.tile * kRows + wave * 32;
   const int row = row_w + col;
   const bool live = row < rows;
   const int tok = min(row, rows - 1) / gq, head = min(row, rows - 1) % gq;
@@ -434,8 +488,8 @@ void paged_prefill_kernel(PrefillParams p) {
 
   // As the table has them, of keys that may lie before or past the sequence: the index is
   // held to the table's row here, the id to the cache where it is used.
-  auto page_at = [&](int key) { return min(max(key, 0) >> p.ps_log2, last_page); };
-  auto find_pages = [&](int j) {
+  auto page_at = [&](int key) MXFA_INLINE { return min(max(key, 0) >> p.ps_log2, last_page); };
+  auto find_pages = [&](int j) MXFA_INLINE {
     const int key0 = k_begin + j * KT;
 #pragma unroll
     for (int u = 0; u < kPages; ++u) {
@@ -457,14 +511,15 @@ void paged_prefill_kernel(PrefillParams p) {
     }
   };
   // Offset in the cache of key's row of this head.
-  auto row_off = [&](int key, int page) -> int64_t {
+  auto row_off = [&](int key, int page) MXFA_INLINE -> int64_t {
     page = min(max(page, 0), p.num_pages - 1);
-    if constexpr (kUniform)
-      return (int64_t)page * p.sp + (head_off + (uint32_t)(key & ps_mask) * (uint64_t)st);
+    if constexpr (kUniform)  // page and token strides within 32 bits, a page's rows too
+      return (int64_t)((uint64_t)(uint32_t)page * (uint32_t)p.sp) +
+             (head_off + (uint32_t)(key & ps_mask) * st);
     return (int64_t)page * p.sp + (int64_t)(key & ps_mask) * p.st + head_off;
   };
   auto load_rows = [&](const char *side, int key0, const int (&pg)[kPages], auto is_k, char *lds,
-                       uint4 (&reg)[kDirect ? 1 : kPer]) {
+                       uint4 (&reg)[kDirect ? 1 : kPer]) MXFA_INLINE {
     if constexpr (kUniform) {
       const char *src = uniform_pointer(side + row_off(key0 + w_row, pg[0]));
       uint32_t at = lds_offset(lds) + w_row * kRowBytes;
@@ -490,7 +545,7 @@ void paged_prefill_kernel(PrefillParams p) {
             side + row_off(key0 + w_row + u * kWaveRows + l_row, pg[u]) + l_chunk * 16);
     }
   };
-  auto load_k_scales = [&](int key0) {
+  auto load_k_scales = [&](int key0) MXFA_INLINE {
     if constexpr (!kWide) {
       if (wave == 0) {
         const int off = (key0 + lane) & ps_mask;
@@ -500,7 +555,7 @@ void paged_prefill_kernel(PrefillParams p) {
       }
     }
   };
-  auto load_tile = [&](int j, int buf) {
+  auto load_tile = [&](int j, int buf) MXFA_INLINE {
     const int key0 = k_begin + j * KT;
     load_rows(p.k, key0 + kAhead, pg_k, std::true_type{}, lds_k[buf], rk);
     load_rows(p.v, key0, pg_v, std::false_type{}, lds_v[buf], rv);
@@ -513,10 +568,22 @@ void paged_prefill_kernel(PrefillParams p) {
       }
     }
   };
-  // Rows from registers to LDS, an 8-bit cache's widened; zeros from row `valid` on.
-  auto store_rows = [&](const uint4 (&reg)[kDirect ? 1 : kPer], char *lds, auto type, auto is_k,
-                        int valid) {
+  // 16 loaded bytes of a row into its LDS row, an 8-bit cache's widened.
+  auto put = [&](auto type, char *dst, const uint4 &w, int sw) MXFA_INLINE {
     using TR = decltype(type);
+    if constexpr (kWide) {
+      *reinterpret_cast<uint4 *>(dst + (l_chunk ^ sw) * 16) = w;
+    } else {
+      const uint2 a = widen_codes<TR, kCache>(w.x), b = widen_codes<TR, kCache>(w.y);
+      const uint2 c = widen_codes<TR, kCache>(w.z), d = widen_codes<TR, kCache>(w.w);
+      *reinterpret_cast<uint4 *>(dst + ((2 * l_chunk) ^ sw) * 16) = make_uint4(a.x, a.y, b.x, b.y);
+      *reinterpret_cast<uint4 *>(dst + ((2 * l_chunk + 1) ^ sw) * 16) =
+          make_uint4(c.x, c.y, d.x, d.y);
+    }
+  };
+  // Rows from registers to LDS; zeros from row `valid` on.
+  auto store_rows = [&](const uint4 (&reg)[kDirect ? 1 : kPer], char *lds, auto type, auto is_k,
+                        int valid) MXFA_INLINE {
     if constexpr (!kDirect) {
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
@@ -527,21 +594,11 @@ void paged_prefill_kernel(PrefillParams p) {
           w = make_uint4(there ? w.x : 0u, there ? w.y : 0u, there ? w.z : 0u, there ? w.w : 0u);
         }
         const int sw = decltype(is_k)::value ? swizzle_k<HD>(r) : swizzle_v<HD>(r);
-        char *dst = lds + r * kRowBytes;
-        if constexpr (kWide) {
-          *reinterpret_cast<uint4 *>(dst + (l_chunk ^ sw) * 16) = w;
-        } else {
-          const uint2 a = widen_codes<TR, kCache>(w.x), b = widen_codes<TR, kCache>(w.y);
-          const uint2 c = widen_codes<TR, kCache>(w.z), d = widen_codes<TR, kCache>(w.w);
-          *reinterpret_cast<uint4 *>(dst + ((2 * l_chunk) ^ sw) * 16) =
-              make_uint4(a.x, a.y, b.x, b.y);
-          *reinterpret_cast<uint4 *>(dst + ((2 * l_chunk + 1) ^ sw) * 16) =
-              make_uint4(c.x, c.y, d.x, d.y);
-        }
+        put(type, lds + r * kRowBytes, w, sw);
       }
     }
   };
-  auto store_k = [&](int buf) {
+  auto store_k = [&](int buf) MXFA_INLINE {
     store_rows(rk, lds_k[buf], T{}, std::true_type{}, KT);
     // A V row without a scale (NaN: it held an infinity or a NaN) takes its key's score along
     // instead, so that it reaches the rows that see the key and no other (a weight of zero
@@ -553,7 +610,7 @@ void paged_prefill_kernel(PrefillParams p) {
   // The loaded rows into LDS (kDirect: they are on their way there; this wave's are waited
   // for). V rows at or past the sequence's end become zeros, whatever their memory holds;
   // their keys are masked.
-  auto store_tile = [&](int j, int buf) {
+  auto store_tile = [&](int j, int buf) MXFA_INLINE {
     const int valid = sq.len - (k_begin + j * KT);  // V rows of the tile that exist
     if constexpr (kDirect) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -581,16 +638,27 @@ void paged_prefill_kernel(PrefillParams p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
 
-  // K operands of the 32 keys in rows r0.. of buffer buf.
-  uint4 kf[NQ];
-  auto read_k = [&](int buf, int r0) {
+  // K operand of the 32 keys in rows r0.. of buffer buf, dims 16 i ..; up to eight are read
+  // ahead of their products.
+  constexpr int kReads = NQ < 8 ? NQ : 8;
+  uint4 kf[kReads];
+  // LDS addresses of the lane's operands, kept in registers where they fit (kUnroll): buffer
+  // and row are then the reads' constant offsets.
+  constexpr bool kUnroll = kDirect && !kExtras;
+  uint32_t k_at[NQ];
 #pragma unroll
-    for (int i = 0; i < NQ; ++i)
-      kf[i] = *reinterpret_cast<const uint4 *>(
-          lds_k[buf] + (r0 + col) * kRowBytes + (((2 * i + half) ^ swizzle_k<HD>(col)) * 16));
+  for (int i = 0; i < NQ; ++i) {
+    k_at[i] = lds_offset(lds_k[0]) + col * kRowBytes + (((2 * i + half) ^ swizzle_k<HD>(col)) * 16);
+    if constexpr (kUnroll) asm("" : "+v"(k_at[i]));
+  }
+  auto read_k = [&](int buf, int r0, int i) MXFA_INLINE {
+    typedef const __attribute__((address_space(3))) u32x4_t LdsVec;
+    const u32x4_t x =
+        *(LdsVec *)(uintptr_t)(k_at[i] + buf * (KT * kRowBytes) + r0 * kRowBytes);
+    kf[i % kReads] = make_uint4(x.x, x.y, x.z, x.w);
   };
   // The scales of an 8-bit cache's rows: scores keys 8 (i / 4) + 4 half + i % 4 of the 32.
-  auto scale_scores = [&](int buf, int r0, f32x16 &s) {
+  auto scale_scores = [&](int buf, int r0, f32x16 &s) MXFA_INLINE {
     if constexpr (!kWide) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -602,14 +670,14 @@ void paged_prefill_kernel(PrefillParams p) {
       }
     }
   };
-  const auto largest = [&](const f32x16 &s) {
+  const auto largest = [&](const f32x16 &s) MXFA_INLINE {
     float x = fmaxf(s[0], s[1]);
 #pragma unroll
     for (int i = 2; i < 16; ++i) x = fmaxf(x, s[i]);
     return x;
   };
   // Options and masks; top: the lane's largest score.
-  auto limit = [&](int key0, f32x16 &s, float &top) {
+  auto limit = [&](int key0, f32x16 &s, float &top) MXFA_INLINE {
     if constexpr (kExtras) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -637,7 +705,7 @@ void paged_prefill_kernel(PrefillParams p) {
     }
   };
   // Moves the reference where a score passed it by more than kPrefillRescaleLog2.
-  auto refer = [&](float top) {
+  auto refer = [&](float top) MXFA_INLINE {
     top *= cs;
     if (__builtin_amdgcn_ballot_w64(top > m + kPrefillRescaleLog2) != 0) {  // wave-uniform
       const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top),
@@ -658,24 +726,28 @@ void paged_prefill_kernel(PrefillParams p) {
   // summed as they come.
   uint32_t pf[8], pl[kSplitP ? 8 : 1];
   float mr;  // the reference; 0 where no key is seen yet (the scores are -inf then)
-  float4 vsc[kWide ? 1 : 4];
-  auto weigh_start = [&](int buf, int r0) {
+  // 8-bit: V's scales of the lane's keys, all read ahead, or (fp16, where the split weights
+  // take the registers) four keys ahead.
+  constexpr int kScales = kSplitP ? 2 : 4;
+  float4 vsc[kScales];
+  auto read_vs = [&](int buf, int r0, int g) MXFA_INLINE {
+    vsc[g % kScales] = *reinterpret_cast<const float4 *>(&lds_vs[buf][r0 + 8 * g + 4 * half]);
+  };
+  auto weigh_start = [&](int buf, int r0) MXFA_INLINE {
     mr = m == -INFINITY ? 0.f : m;
     if constexpr (!kWide) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        vsc[g] = *reinterpret_cast<const float4 *>(&lds_vs[buf][r0 + 8 * g + 4 * half]);
+      for (int g = 0; g < kScales - (kSplitP ? 1 : 0); ++g) read_vs(buf, r0, g);
     }
   };
-  auto weigh = [&](auto ic, f32x16 &s) {
+  auto weigh = [&](auto ic, int buf, int r0, f32x16 &s) MXFA_INLINE {
     constexpr int i = decltype(ic)::value;
     s[i] = fast_exp2(__builtin_fmaf(s[i], cs, -mr));
     if constexpr (!kWide) {
+      if constexpr (kSplitP && i % 4 == 0 && i < 12) read_vs(buf, r0, i / 4 + 1);
       l += s[i];
-      s[i] *= (i & 3) == 0 ? vsc[i >> 2].x
-              : (i & 3) == 1 ? vsc[i >> 2].y
-              : (i & 3) == 2 ? vsc[i >> 2].z
-                             : vsc[i >> 2].w;
+      const float4 f = vsc[(i >> 2) % kScales];
+      s[i] *= (i & 3) == 0 ? f.x : (i & 3) == 1 ? f.y : (i & 3) == 2 ? f.z : f.w;
     }
     if constexpr (i & 1) {
       pf[i >> 1] = Prod32<TV>::pack(s[i - 1], s[i]);
@@ -691,15 +763,21 @@ void paged_prefill_kernel(PrefillParams p) {
   // 4 (l / 32) + (l / 4) % 4 and receives dim l % 32 of four keys.
   const int v_key = 4 * half + ((lane >> 2) & 3);
   const int v_dim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);  // within the 32-dim block
-  auto read_v = [&](int buf, int r0, int d) {
+  uint32_t v_at[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    const int byte = (d * 32 + v_dim) * 2;
+    v_at[d] = lds_offset(lds_v[0]) + v_key * kRowBytes +
+              (((byte >> 4) ^ swizzle_v<HD>(v_key)) << 4) + (byte & 15);
+    if constexpr (kUnroll) asm("" : "+v"(v_at[d]));
+  }
+  auto read_v = [&](int buf, int r0, int d) MXFA_INLINE {
     uint32_t w[4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int byte = (d * 32 + v_dim) * 2;
-      const int at = (r0 + 8 * u + v_key) * kRowBytes +
-                     (((byte >> 4) ^ swizzle_v<HD>(v_key)) << 4) + (byte & 15);
+      const uint32_t at = v_at[d] + buf * (KT * kRowBytes) + (r0 + 8 * u) * kRowBytes;
       typedef __attribute__((address_space(3))) s16x4v LdsVec;
-      const s16x4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec *)(lds_v[buf] + at));
+      const s16x4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsVec *)(uintptr_t)at);
       const uint2 y = __builtin_bit_cast(uint2, x);
       w[2 * u] = y.x;
       w[2 * u + 1] = y.y;
@@ -711,18 +789,21 @@ void paged_prefill_kernel(PrefillParams p) {
   // product. The order is written out (sched_barrier): left to itself the compiler issues
   // the products in a row, and a wave issues in order.
   float top = -INFINITY;
-  auto first_scores = [&](int buf, int r0, f32x16 &s) {
-    read_k(buf, r0);
+  auto first_scores = [&](int buf, int r0, f32x16 &s) MXFA_INLINE {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < NQ; ++i) s = Prod32<T>::run(kf[i], qf[i], s);
+    for (int i = 0; i < NQ; ++i) {
+      read_k(buf, r0, i);
+      s = Prod32<T>::run(kf[i % kReads], qf[i], s);
+    }
     scale_scores(buf, r0, s);
     if constexpr (!kExtras) top = largest(s);
   };
   // The weights of cur's keys and their part of the output, and nxt's scores.
-  auto advance = [&](int buf, int r0, f32x16 &cur, f32x16 &nxt) {
-    read_k(buf, r0);
+  auto advance = [&](int buf, int r0, f32x16 &cur, f32x16 &nxt) MXFA_INLINE {
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) read_k(buf, r0, i);
     weigh_start(buf, r0);
     uint4 vf[ND];
     __builtin_amdgcn_sched_barrier(0);
@@ -730,9 +811,10 @@ void paged_prefill_kernel(PrefillParams p) {
     for (int i = 0; i < 16; ++i) nxt[i] = 0.f;
     static_unroll<NQ>([&](auto ic) {
       constexpr int i = decltype(ic)::value;
-      nxt = Prod32<T>::run(kf[i], qf[i], nxt);
+      nxt = Prod32<T>::run(kf[i % kReads], qf[i], nxt);
+      if constexpr (i + kReads < NQ) read_k(buf, r0, i + kReads);
       static_unroll<16 / NQ>([&](auto jc) {
-        weigh(std::integral_constant<int, i * (16 / NQ) + decltype(jc)::value>{}, cur);
+        weigh(std::integral_constant<int, i * (16 / NQ) + decltype(jc)::value>{}, buf, r0, cur);
       });
       if constexpr (i >= NQ / 2) {  // the first V operands, in the second half's shadow
         static_unroll<2 * ND / NQ>([&](auto jc) {
@@ -760,14 +842,111 @@ void paged_prefill_kernel(PrefillParams p) {
     }
     if constexpr (!kExtras) top = largest(nxt);
   };
-  auto step = [&](int key0, int buf, int r0, f32x16 &cur, f32x16 &nxt) {
+  auto step = [&](int key0, int buf, int r0, f32x16 &cur, f32x16 &nxt) MXFA_INLINE {
     if (key0 <= any_to) {  // some row of the wave sees some of the 32 keys
       limit(key0, cur, top);
       refer(top);
       advance(buf, r0, cur, nxt);  // (past the last keys, products that nobody looks at)
     }
   };
-  if (j0 < j1) {
+  if (sq.few) {
+    // Few rows: the four waves share them and each takes a quarter of the piece's keys, 32 at
+    // a time through its own quarter of the K and V buffers, with no barrier; rows come
+    // through registers, the next 32 keys' loads in flight during the math. (One wave on all
+    // keys is bound by the time of a step: 31 sequences of one token on 1k-8k int8 keys beside
+    // a chunk of 1024, 32q/8kv HD 128, 179 us against the figure in launch_prefill_t.)
+    constexpr int kFew = 32 / kWaveRows;
+    constexpr int kFewPages = kUniform ? 2 : kFew;
+    char *const own_k = lds_k[wave >> 1] + (wave & 1) * 32 * kRowBytes;
+    char *const own_v = lds_v[wave >> 1] + (wave & 1) * 32 * kRowBytes;
+    const int buf = wave >> 1, r0 = (wave & 1) * 32;
+    const int blocks = 2 * (j1 - j0);
+    const int i1 = blocks * (wave + 1) / kPrefillWaves;
+    const int base = k_begin + j0 * KT;
+    uint4 fk[kFew], fv[kFew];
+    int pages[kFewPages], page_s = 0;
+    float fks = 1.f, fvs = 1.f;
+    auto few_pages = [&](int i) MXFA_INLINE {
+      const int key0 = base + 32 * i;
+#pragma unroll
+      for (int u = 0; u < kFewPages; ++u) {
+        if constexpr (kUniform)
+          pages[u] =
+              ((const __attribute__((address_space(4))) int32_t *)bt)[page_at(key0 + 16 * u)];
+        else
+          pages[u] = bt[page_at(key0 + u * kWaveRows + l_row)];
+      }
+      if constexpr (!kWide) page_s = bt[page_at(key0 + (lane & 31))];
+    };
+    auto few_load = [&](int i) MXFA_INLINE {
+      const int key0 = base + 32 * i;
+#pragma unroll
+      for (int u = 0; u < kFew; ++u) {
+        const int r = u * kWaveRows;
+        int64_t off;
+        if constexpr (kUniform)
+          off = row_off(key0 + r, pages[r >> 4]) + lane_off;
+        else
+          off = row_off(key0 + r + l_row, pages[u]);
+        off += l_chunk * 16;
+        fk[u] = load_stream16(p.k + off);
+        fv[u] = load_stream16(p.v + off);
+      }
+      if constexpr (!kWide) {
+        const int64_t page = min(max(page_s, 0), p.num_pages - 1);
+        const int at = (key0 + (lane & 31)) & ps_mask;
+        fks = p.ks ? p.ks[page * p.ks_sp + (int64_t)kvh * p.ks_sh + at] : 1.f;
+        fvs = p.vs ? p.vs[page * p.vs_sp + (int64_t)kvh * p.vs_sh + at] : 1.f;
+      }
+    };
+    int i = blocks * wave / kPrefillWaves;
+    if (i < i1) {
+      few_pages(i);
+      few_load(i);
+      few_pages(i + 1);
+    }
+    for (; i < i1; ++i) {
+      const int key0 = base + 32 * i;
+#pragma unroll
+      for (int u = 0; u < kFew; ++u) {
+        const int r = u * kWaveRows + l_row;
+        const bool there = key0 + r < sq.len;
+        put(T{}, own_k + r * kRowBytes, fk[u], swizzle_k<HD>(r));
+        const uint4 w = fv[u];
+        put(TV{}, own_v + r * kRowBytes,
+            make_uint4(there ? w.x : 0u, there ? w.y : 0u, there ? w.z : 0u, there ? w.w : 0u),
+            swizzle_v<HD>(r));
+      }
+      if constexpr (!kWide) {
+        if (lane < 32) {
+          const bool whole = fabsf(fvs) < INFINITY;
+          lds_ks[buf][r0 + lane] = whole ? fks : __builtin_nanf("");
+          lds_vs[buf][r0 + lane] = whole && key0 + lane < sq.len ? fvs : 0.f;
+        }
+      }
+      if (i + 1 < i1) {
+        few_load(i + 1);
+        few_pages(i + 2);
+      }
+      f32x16 s;
+      first_scores(buf, r0, s);
+      limit(key0, s, top);
+      refer(top);
+      weigh_start(buf, r0);
+      static_unroll<16>([&](auto ic) { weigh(ic, buf, r0, s); });
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const uint4 a = read_v(buf, r0 + 16 * st, d);
+          o[d] = Prod32<TV>::run(
+              a, make_uint4(pf[4 * st], pf[4 * st + 1], pf[4 * st + 2], pf[4 * st + 3]), o[d]);
+          if constexpr (kSplitP)
+            o[d] = Prod32<TV>::run(
+                a, make_uint4(pl[4 * st], pl[4 * st + 1], pl[4 * st + 2], pl[4 * st + 3]), o[d]);
+        }
+    }
+  } else if (j0 < j1) {
     f32x16 sa, sb;
     // K's stage before the first holds the first 32 keys.
     find_pages(j0 - 1);
@@ -780,8 +959,8 @@ void paged_prefill_kernel(PrefillParams p) {
     if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     first_scores(1, kAhead, sa);
-    for (int j = j0; j < j1; ++j) {
-      const int buf = (j - j0) & 1, key0 = k_begin + j * KT;
+    auto tile = [&](int j, auto bc) MXFA_INLINE {
+      const int buf = bc, key0 = k_begin + j * KT;
       // One barrier a tile: past it V of tile j and K 32 keys on are in LDS, and every wave is
       // done with the other buffers, which the next loads fill.
       store_tile(j, buf);
@@ -796,12 +975,88 @@ void paged_prefill_kernel(PrefillParams p) {
       }
       step(key0, buf, 0, sa, sb);
       step(key0 + 32, buf, 32, sb, sa);
+    };
+    if constexpr (kUnroll) {
+      // Two tiles a round: the buffers are then constants, and part of the LDS reads' offsets.
+      for (int j = j0; j < j1; j += 2) {
+        tile(j, std::integral_constant<int, 0>{});
+        if (j + 1 < j1) tile(j + 1, std::integral_constant<int, 1>{});
+      }
+    } else {  // (the staging registers leave no room for that)
+      for (int j = j0; j < j1; ++j) tile(j, (j - j0) & 1);
     }
   }
 
   const auto lw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false,
                                                    false);
   l = __uint_as_float(lw[0]) + __uint_as_float(lw[1]);
+  if (sq.few) {
+    // The four waves' rows: references and sums, then the accumulators as [4 dims][row] through
+    // the K (waves 0, 1) and V (2, 3) buffers; thread (part, row) then joins HD / 8 dims of a
+    // row in wave order.
+    __syncthreads();
+    float4 *const mine = reinterpret_cast<float4 *>(wave < 2 ? lds_k[0] : lds_v[0]) +
+                         (wave & 1) * (HD / 4) * 32;
+    if (half == 0) {
+      few_m[wave][col] = m;
+      few_l[wave][col] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        mine[(d * 8 + 2 * g + half) * 32 + col] =
+            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    __syncthreads();
+    const int r = threadIdx.x & 31, part = threadIdx.x >> 5;
+    if (r >= rows) return;
+    float mm = -INFINITY, ll = 0.f, f[kPrefillWaves];
+#pragma unroll
+    for (int w = 0; w < kPrefillWaves; ++w) mm = fmaxf(mm, few_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kPrefillWaves; ++w) {
+      // A wave that saw no key has the reference -inf and no sum; one that saw only NaN too,
+      // and its NaN sum stays.
+      f[w] = few_m[w][r] == -INFINITY ? 1.f : fast_exp2(few_m[w][r] - mm);
+      ll += f[w] * few_l[w][r];
+    }
+    const int64_t at = (int64_t)it.slot * p.hkv + kvh;
+    float inv;
+    if (it.pieces > 1) {
+      if (threadIdx.x == 0)
+        p.ws_desc[at] = make_int4(it.piece == 0 ? it.pieces : 0, it.b, it.tile, 0);
+      if (part == 0)
+        p.ws_lse[at * kRows + r] = ll > 0.f ? mm + __log2f(ll) : (ll == 0.f ? -INFINITY : ll);
+      inv = ll == 0.f ? 0.f : v_scale / ll;
+    } else {
+      float den = ll;
+      if (p.sinks) den += fast_exp2(p.sinks[kvh * gq + r % gq] * kPrefillLog2e - mm);
+      inv = ll == 0.f ? 0.f : v_scale / den;
+    }
+    char *const dst = p.out + (int64_t)(sq.start + r / gq) * p.o_st +
+                      (int64_t)(kvh * gq + r % gq) * p.o_sh;
+#pragma unroll
+    for (int cc = 0; cc < HD / 32; ++cc) {
+      const int chunk = part * (HD / 32) + cc;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kPrefillWaves; ++w) {
+        const float4 x = (reinterpret_cast<const float4 *>(w < 2 ? lds_k[0] : lds_v[0]) +
+                          (w & 1) * (HD / 4) * 32)[chunk * 32 + r];
+        acc.x += f[w] * x.x;
+        acc.y += f[w] * x.y;
+        acc.z += f[w] * x.z;
+        acc.w += f[w] * x.w;
+      }
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (it.pieces > 1)
+        *reinterpret_cast<float4 *>(p.ws_o + (at * kRows + r) * HD + 4 * chunk) = acc;
+      else
+        *reinterpret_cast<uint2 *>(dst + 8 * chunk) =
+            make_uint2(Prod32<T>::pack(acc.x, acc.y), Prod32<T>::pack(acc.z, acc.w));
+    }
+    return;
+  }
   if (it.pieces > 1) {
     const int64_t at = (int64_t)it.slot * p.hkv + kvh;
     if (threadIdx.x == 0)
@@ -850,7 +1105,7 @@ __global__ __launch_bounds__(kPrefillJoinThreads) void paged_prefill_join_kernel
   const int4 d = p.ws_desc[at];
   const int pieces = d.x;
   if (pieces <= 1 || slot + pieces > p.max_slots || d.y < 0 || d.y >= p.batch) return;
-  const PrefillSeq sq = prefill_seq<kRows>(p, d.y);
+  const PrefillSeq sq = prefill_seq(p, d.y);
   const int chunk = threadIdx.x % (HD / 4);
   const int rows = min(kRows, sq.n * p.gq - d.z * kRows);
   for (int r = blockIdx.y * kJoinRows + threadIdx.x / (HD / 4); r < rows;

@@ -491,20 +491,6 @@ __device__ __forceinline__ float head_of_row(float x, int row) {
   return v;
 }
 
-// Inclusive prefix sum over the 64 lanes of a wave with DPP moves only (no
-// LDS permutes): a Hillis-Steele scan inside each 16-lane row (row_shr 1, 2,
-// 4, 8), then the row totals carried across rows (row_bcast:15 into rows 1
-// and 3, row_bcast:31 into rows 2 and 3). Lanes a move leaves unwritten add 0.
-__device__ __forceinline__ int wave_scan_incl(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 1, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 2, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 4, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, kDppRowShr0 + 8, 0xf, 0xf, true);
-  x += __builtin_amdgcn_update_dpp(0, x, kDppRowBcast15, 0xa, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, kDppRowBcast31, 0xc, 0xf, false);
-  return x;
-}
-
 // Exclusive prefix sum of per-sequence tile counts into s[0..B] (LDS), all
 // threads (seqlens and B are the kernel's preloaded leading arguments, equal
 // to p.seqlens and p.batch). The lengths are read from memory once, eight loads in flight per
