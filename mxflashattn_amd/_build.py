@@ -105,9 +105,10 @@ _REMARK = re.compile(r"remark:\s+(Function Name|VGPRs Spill|ScratchSize \[bytes/
 # Dynamic LDS (the tile prefix sums, the per-sequence kernel's pieces) is not
 # counted in the remark.
 # (The prefill's tiles: two buffers of K and of V, 64 rows of up to 512 bytes, their
-# scales, and its work search.)
+# scales, and its work search; the places of the rows that a block reads back.)
 STATIC_LDS_LIMITS = {"split_combine_kernel": 256 * 6 * 4,
-                     "paged_prefill_kernel": 4 * 64 * 512 + 4096}
+                     "paged_prefill_kernel": 4 * 64 * 512 + 4096,
+                     "gather_cache_kernel": 16 * 12}
 STATIC_LDS_DEFAULT = 64
 
 

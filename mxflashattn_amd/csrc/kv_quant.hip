@@ -59,51 +59,77 @@ __device__ __forceinline__ float row_scale(uint32_t top) {
   return finite ? s : __builtin_nanf("");
 }
 
+// x / s correctly rounded from y = 1 / s correctly rounded: with q = x y off by an ulp at
+// most, the residual x - q s is exact in one fma, and q plus the residual times y rounds to
+// the quotient's nearest (Markstein's theorem). Exact where the residual is no subnormal
+// number, so for |x| of 2^-100 or more; below that (s is then the larger by far, see kFastScale)
+// the quotient is so small that its code is 0 either way.
+__device__ __forceinline__ float quotient(float x, float s, float y) {
+  const float q = x * y;
+  return __builtin_fmaf(__builtin_fmaf(-q, s, x), y, q);
+}
+// Rows of smaller scales take the division itself. Three instructions an element instead of
+// ten: 16384 rows of 8 x 128, bf16 to e4m3fn, 28.7 -> 20.7 us on MI355X (102 MB, 4.9 TB/s; a
+// large copy reaches 4.8).
+constexpr float kFastScale = 0x1p-60f;
+
+// Four codes of x / s. No quotient needs a clamp: |x| <= TOP s (1 + 2^-23), which rounds to
+// TOP or less.
 template <bool kInt8>
-__device__ __forceinline__ uint32_t quad_codes(float a, float b, float c, float d, float s) {
+__device__ __forceinline__ uint32_t quad_codes(float a, float b, float c, float d) {
   if constexpr (kInt8) {
-    const auto one = [&](float x) {
-      return (uint32_t)(int)fminf(fmaxf(__builtin_rintf(__fdiv_rn(x, s)), -127.f), 127.f) & 0xffu;
-    };
-    return one(a) | (one(b) << 8) | (one(c) << 16) | (one(d) << 24);
+    const auto one = [&](float x) { return (uint32_t)(int)__builtin_rintf(x); };
+    const uint32_t lo = __builtin_amdgcn_perm(one(b), one(a), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(one(d), one(c), 0x04000c0cu);
+    return lo | hi;
   } else {
-    const auto one = [&](float x) { return fminf(fmaxf(__fdiv_rn(x, s), -448.f), 448.f); };
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(one(a), one(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(one(c), one(d), r, true);
+    const int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
   }
 }
 
 template <typename T, bool kInt8>
 __device__ __forceinline__ uint2 row_codes(const uint4 w, float s) {
   using E = Elem<T>;
-  if (s != s) return make_uint2(0u, 0u);
-  return make_uint2(
-      quad_codes<kInt8>(E::lo(w.x), E::hi(w.x), E::lo(w.y), E::hi(w.y), s),
-      quad_codes<kInt8>(E::lo(w.z), E::hi(w.z), E::lo(w.w), E::hi(w.w), s));
+  float x[8] = {E::lo(w.x), E::hi(w.x), E::lo(w.y), E::hi(w.y),
+                E::lo(w.z), E::hi(w.z), E::lo(w.w), E::hi(w.w)};
+  if (s >= kFastScale) {
+    const float y = __fdiv_rn(1.f, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = quotient(x[i], s, y);
+  } else {
+    // (s = NaN: codes 0)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = s != s ? 0.f : __fdiv_rn(x[i], s);
+  }
+  return make_uint2(quad_codes<kInt8>(x[0], x[1], x[2], x[3]),
+                    quad_codes<kInt8>(x[4], x[5], x[6], x[7]));
 }
 
 // A group of 2^lanes_log2 lanes (the power of two at or above HD / 8) takes one row of one
 // head, K and V, so its largest element is a few exchanges inside the wave.
-template <typename T, bool kInt8>
+// I = uint32_t (calls of fewer rows x heads than 2^31 less a step): divisions in 32 bits.
+template <typename T, bool kInt8, typename I>
 __global__ __launch_bounds__(kQuantThreads) void quantize_and_cache_kernel(QuantParams p) {
   const int lanes = 1 << p.lanes_log2;
   const int f = threadIdx.x & (lanes - 1);
-  const int64_t total = (int64_t)p.rows * p.hkv;
-  const int64_t step = (int64_t)gridDim.x * (kQuantThreads >> p.lanes_log2);
-  for (int64_t i = (int64_t)blockIdx.x * (kQuantThreads >> p.lanes_log2) +
-                   (threadIdx.x >> p.lanes_log2);
+  const I total = (I)p.rows * (I)p.hkv;
+  const I step = (I)gridDim.x * (I)(kQuantThreads >> p.lanes_log2);
+  for (I i = (I)blockIdx.x * (I)(kQuantThreads >> p.lanes_log2) +
+             (I)(threadIdx.x >> p.lanes_log2);
        i < total; i += step) {
-    const int r = (int)(i / p.hkv), h = (int)(i - (int64_t)r * p.hkv);
+    const int r = (int)(i / (I)p.hkv), h = (int)(i - (I)r * (I)p.hkv);
+    // The row's loads go out with the slot's: they do not depend on it.
     const int64_t slot = p.slots[r];
-    const int64_t page = slot >> p.ps_log2;
-    if (slot < 0 || page >= p.num_pages) continue;  // the same for the whole group
-    const int off = (int)(slot & ((1 << p.ps_log2) - 1));
     uint4 wk = make_uint4(0u, 0u, 0u, 0u), wv = wk;
     if (f < p.frags) {
       const int64_t src = (int64_t)r * p.s_t + (int64_t)h * p.s_h + f * 8;
       wk = *reinterpret_cast<const uint4 *>(p.k + src);
       wv = *reinterpret_cast<const uint4 *>(p.v + src);
     }
+    const int64_t page = slot >> p.ps_log2;
+    if (slot < 0 || page >= p.num_pages) continue;  // the same for the whole group
+    const int off = (int)(slot & ((1 << p.ps_log2) - 1));
     const float ks = row_scale<T, kInt8>(row_top<T>(wk, lanes));
     const float vs = row_scale<T, kInt8>(row_top<T>(wv, lanes));
     if (f < p.frags) {
@@ -172,15 +198,22 @@ __device__ __forceinline__ uint4 read_codes(uint2 c, float s) {
   return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
+// A block takes kGatherRows consecutive rows: threads 0.. find each row's sequence (a binary
+// search of the offsets) and place, in LDS, then all threads move the rows, 16 bytes of the
+// narrower side of K and of V each, their loads all out before the first store. Against a
+// thread that searched for its own eight codes: 16 sequences of 1k-8k int8 rows, 8 x 128,
+// 138 -> 95 us on MI355X (437 MB, 4.6 TB/s).
 // kBits 16: the cache holds T itself; 8: codes (kInt8 or e4m3fn).
+constexpr int kGatherRows = 16;
+
 template <typename T, int kBits, bool kInt8>
 __global__ __launch_bounds__(kQuantThreads) void gather_cache_kernel(GatherParams p) {
-  const int units = p.hkv * p.frags;
-  const int64_t all = (int64_t)p.total * units;
-  const int64_t step = (int64_t)gridDim.x * kQuantThreads;
-  for (int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x; i < all; i += step) {
-    const int r = (int)(i / units), u = (int)(i - (int64_t)r * units);
-    const int h = u / p.frags, f = u - h * p.frags;
+  __shared__ int64_t s_page[kGatherRows];  // -1: a row of no sequence
+  __shared__ int s_off[kGatherRows];
+  const int r0 = blockIdx.x * kGatherRows;
+  const int rows = min(kGatherRows, p.total - r0);
+  if ((int)threadIdx.x < rows) {
+    const int r = r0 + threadIdx.x;
     // The last sequence that starts at or before row r.
     int lo = 0, n = p.batch;
     while (n > 1) {
@@ -190,25 +223,60 @@ __global__ __launch_bounds__(kQuantThreads) void gather_cache_kernel(GatherParam
       n = right ? n - half : half;
     }
     const int pos = r - p.cu[lo];
-    if (pos < 0 || r >= p.cu[lo + 1]) continue;
     const int pidx = pos >> p.ps_log2;
-    if (pidx >= p.btw) continue;
-    const int64_t page = min(max(p.bt[(int64_t)lo * p.bt_stride + pidx], 0), p.num_pages - 1);
-    const int off = pos & ((1 << p.ps_log2) - 1);
-    const int64_t src = page * p.c_sp + (int64_t)off * p.c_st + (int64_t)h * p.c_sh +
-                        f * (kBits == 16 ? 16 : 8);
-    const int64_t dst = (int64_t)r * p.o_st + (int64_t)h * p.o_sh + f * 8;
-    if constexpr (kBits == 16) {
-      *reinterpret_cast<uint4 *>(p.ko + dst) = *reinterpret_cast<const uint4 *>(p.kc + src);
-      *reinterpret_cast<uint4 *>(p.vo + dst) = *reinterpret_cast<const uint4 *>(p.vc + src);
-    } else {
-      float ks = p.k_scale ? p.k_scale[0] : 1.f, vs = p.v_scale ? p.v_scale[0] : 1.f;
-      if (p.ks) ks = p.ks[page * p.ks_sp + (int64_t)h * p.ks_sh + off];
-      if (p.vs) vs = p.vs[page * p.vs_sp + (int64_t)h * p.vs_sh + off];
-      const uint2 ck = *reinterpret_cast<const uint2 *>(p.kc + src);
-      const uint2 cv = *reinterpret_cast<const uint2 *>(p.vc + src);
-      *reinterpret_cast<uint4 *>(p.ko + dst) = read_codes<T, kInt8>(ck, ks);
-      *reinterpret_cast<uint4 *>(p.vo + dst) = read_codes<T, kInt8>(cv, vs);
+    int64_t page = -1;
+    if (pos >= 0 && r < p.cu[lo + 1] && pidx < p.btw)
+      page = min(max(p.bt[(int64_t)lo * p.bt_stride + pidx], 0), p.num_pages - 1);
+    s_page[threadIdx.x] = page;
+    s_off[threadIdx.x] = pos & ((1 << p.ps_log2) - 1);
+  }
+  __syncthreads();
+  constexpr int kElems = kBits == 16 ? 8 : 16;  // of a thread's 16 bytes
+  const int frags = p.frags / (kElems / 8);     // of a row
+  const int units = p.hkv * frags;              // of a token
+  const int all = rows * units;
+  constexpr int kAhead = 4;
+  for (int i0 = threadIdx.x; i0 < all; i0 += kAhead * kQuantThreads) {
+    uint4 ck[kAhead], cv[kAhead];
+    float ks[kAhead], vs[kAhead];
+    int64_t dst[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int i = min(i0 + a * kQuantThreads, all - 1);
+      const int row = i / units, u = i - row * units;
+      const int h = u / frags, f = u - h * frags;
+      const int64_t page = s_page[row];
+      const int off = s_off[row];
+      dst[a] = page < 0 || i0 + a * kQuantThreads >= all
+                   ? -1
+                   : (int64_t)(r0 + row) * p.o_st + (int64_t)h * p.o_sh + f * kElems;
+      const int64_t at = max(page, (int64_t)0);
+      const int64_t src = at * p.c_sp + (int64_t)off * p.c_st + (int64_t)h * p.c_sh + f * 16;
+      ck[a] = load_stream16(p.kc + src);
+      cv[a] = load_stream16(p.vc + src);
+      if constexpr (kBits == 8) {
+        ks[a] = p.ks   ? p.ks[at * p.ks_sp + (int64_t)h * p.ks_sh + off]
+                : p.k_scale ? p.k_scale[0]
+                            : 1.f;
+        vs[a] = p.vs   ? p.vs[at * p.vs_sp + (int64_t)h * p.vs_sh + off]
+                : p.v_scale ? p.v_scale[0]
+                            : 1.f;
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      if (dst[a] < 0) continue;
+      uint4 *const k = reinterpret_cast<uint4 *>(p.ko + dst[a]);
+      uint4 *const v = reinterpret_cast<uint4 *>(p.vo + dst[a]);
+      if constexpr (kBits == 16) {
+        *k = ck[a];
+        *v = cv[a];
+      } else {
+        k[0] = read_codes<T, kInt8>(make_uint2(ck[a].x, ck[a].y), ks[a]);
+        k[1] = read_codes<T, kInt8>(make_uint2(ck[a].z, ck[a].w), ks[a]);
+        v[0] = read_codes<T, kInt8>(make_uint2(cv[a].x, cv[a].y), vs[a]);
+        v[1] = read_codes<T, kInt8>(make_uint2(cv[a].z, cv[a].w), vs[a]);
+      }
     }
   }
 }
@@ -284,10 +352,18 @@ int mxfa_package_quantize_and_cache_launch(
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kQuantThreads), 0, (hipStream_t)stream, p);
   };
   const bool i8 = cache_dtype == MXFA_PACKAGE_DTYPE_INT8;
+  const auto pick = [&](auto type, auto codes) {
+    using T = decltype(type);
+    constexpr bool kInt8 = decltype(codes)::value;
+    if ((int64_t)num_tokens * kv_heads < ((int64_t)1 << 31) - ((int64_t)1 << 24))
+      go(quantize_and_cache_kernel<T, kInt8, uint32_t>);
+    else
+      go(quantize_and_cache_kernel<T, kInt8, int64_t>);
+  };
   if (dtype == MXFA_DTYPE_BF16)
-    i8 ? go(quantize_and_cache_kernel<BF16, true>) : go(quantize_and_cache_kernel<BF16, false>);
+    i8 ? pick(BF16{}, std::true_type{}) : pick(BF16{}, std::false_type{});
   else
-    i8 ? go(quantize_and_cache_kernel<F16, true>) : go(quantize_and_cache_kernel<F16, false>);
+    i8 ? pick(F16{}, std::true_type{}) : pick(F16{}, std::false_type{});
   return hipGetLastError() == hipSuccess ? MXFA_OK : MXFA_ELAUNCH;
 }
 
@@ -353,7 +429,7 @@ int mxfa_package_gather_cache_launch(
   p.frags = head_dim / 8;
   p.ps_log2 = ps;
   p.num_pages = num_pages;
-  const unsigned blocks = blocks_for((int64_t)total * kv_heads * p.frags);
+  const unsigned blocks = (unsigned)(((int64_t)total + kGatherRows - 1) / kGatherRows);
   const auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kQuantThreads), 0, (hipStream_t)stream, p);
   };
