@@ -319,6 +319,7 @@ int mxfa_package_quantize_and_cache_launch(
   if (!al(key, 16) || !al(value, 16) || !al(k_cache, 16) || !al(v_cache, 16) ||
       !al(k_scales, 4) || !al(v_scales, 4) || !al(slot_mapping, 8))
     return MXFA_EINVAL;
+  if (k_cache == v_cache || k_scales == v_scales) return MXFA_EINVAL;
   if (((kv_stride_token | kv_stride_head) & 7) || kv_stride_token < 0 || kv_stride_head < 0 ||
       ((cache_stride_page | cache_stride_token | cache_stride_head) & 15) ||
       cache_stride_page < 0 || cache_stride_token < 0 || cache_stride_head < 0 ||
@@ -397,6 +398,7 @@ int mxfa_package_gather_cache_launch(
       bt_stride < 0)
     return MXFA_EINVAL;
   // Rows of the outputs are written by different threads: none may share memory.
+  if (k_out == v_out) return MXFA_EINVAL;
   if (((out_stride_token | out_stride_head) & 7) || (kv_heads > 1 && out_stride_head < head_dim) ||
       (total > 1 && out_stride_token < (kv_heads - 1) * out_stride_head + head_dim))
     return MXFA_EINVAL;

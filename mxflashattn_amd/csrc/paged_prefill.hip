@@ -160,7 +160,9 @@ int mxfa_package_prefill_launch(
   p.scale = scale;
   p.softcap = softcap;
   p.causal = causal != 0;
-  p.window_left = window_left;
+  // A window over every position that a table holds hides nothing (and stays clear of the end
+  // of 32 bits).
+  p.window_left = window_left < max_len ? window_left : -1;
   p.batch = batch;
   p.rows_q = rows_q;
   p.hkv = kv_heads;

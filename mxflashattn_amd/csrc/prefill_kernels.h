@@ -239,7 +239,7 @@ __device__ __forceinline__ int prefill_pieces(const PrefillSeq &q, int most) {
 // the pieces of cut tiles within 2 * target.
 __device__ __forceinline__ int prefill_most(const PrefillParams &p, float work) {
   if (p.target <= 0) return 0x7fffffff;
-  return max(p.least, (int)fminf(work * 1.001f / (float)p.target + 1.f, 1e9f));
+  return max(p.least, (int)fminf(work * 1.001f / (float)p.target + 1.f, 2e9f));
 }
 
 struct PrefillItem {
@@ -412,12 +412,13 @@ void paged_prefill_kernel(PrefillParams p) {
   const int rows = sq.n * gq;  // of the sequence, per kv head
   const int first_pos = sq.len - sq.n;
 
-  // Keys of the tile, then of the piece, in tiles of KT.
+  // Keys that some row of the tile sees, [k_first, k_end), then tiles of KT of them, then the
+  // piece's.
   const int t_first = it.tile * kRows / gq;
   const int t_last = min(sq.n - 1, (it.tile * kRows + kRows - 1) / gq);
   const int k_end = max(0, p.causal ? min(sq.len, first_pos + t_last + 1) : sq.len);
-  const int k_begin =
-      p.window_left >= 0 ? max(0, first_pos + t_first - p.window_left) / KT * KT : 0;
+  const int k_first = p.window_left >= 0 ? max(0, first_pos + t_first - p.window_left) : 0;
+  const int k_begin = k_first / KT * KT;
   const int all = k_end > k_begin ? (k_end - k_begin + KT - 1) / KT : 0;
   const int j0 = (int)((int64_t)all * it.piece / it.pieces);
   const int j1 = (int)((int64_t)all * (it.piece + 1) / it.pieces);
@@ -581,16 +582,16 @@ void paged_prefill_kernel(PrefillParams p) {
           make_uint4(c.x, c.y, d.x, d.y);
     }
   };
-  // Rows from registers to LDS; zeros from row `valid` on.
+  // Rows from registers to LDS; of V, zeros outside rows [lo, hi).
   auto store_rows = [&](const uint4 (&reg)[kDirect ? 1 : kPer], char *lds, auto type, auto is_k,
-                        int valid) MXFA_INLINE {
+                        int lo, int hi) MXFA_INLINE {
     if constexpr (!kDirect) {
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
         const int r = w_row + u * kWaveRows + l_row;
         uint4 w = reg[u];
         if constexpr (!decltype(is_k)::value) {
-          const bool there = r < valid;
+          const bool there = r >= lo && r < hi;
           w = make_uint4(there ? w.x : 0u, there ? w.y : 0u, there ? w.z : 0u, there ? w.w : 0u);
         }
         const int sw = decltype(is_k)::value ? swizzle_k<HD>(r) : swizzle_v<HD>(r);
@@ -599,7 +600,7 @@ void paged_prefill_kernel(PrefillParams p) {
     }
   };
   auto store_k = [&](int buf) MXFA_INLINE {
-    store_rows(rk, lds_k[buf], T{}, std::true_type{}, KT);
+    store_rows(rk, lds_k[buf], T{}, std::true_type{}, 0, KT);
     // A V row without a scale (NaN: it held an infinity or a NaN) takes its key's score along
     // instead, so that it reaches the rows that see the key and no other (a weight of zero
     // times NaN would).
@@ -608,25 +609,25 @@ void paged_prefill_kernel(PrefillParams p) {
     }
   };
   // The loaded rows into LDS (kDirect: they are on their way there; this wave's are waited
-  // for). V rows at or past the sequence's end become zeros, whatever their memory holds;
-  // their keys are masked.
+  // for). V rows that no row of the tile sees (past its last key, ahead of its windows) become
+  // zeros, whatever their memory holds: a weight of zero times a NaN is a NaN.
   auto store_tile = [&](int j, int buf) MXFA_INLINE {
-    const int valid = sq.len - (k_begin + j * KT);  // V rows of the tile that exist
+    const int lo = k_first - (k_begin + j * KT), hi = k_end - (k_begin + j * KT);
     if constexpr (kDirect) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (valid < KT) {  // once a sequence
+      if (hi < KT || lo > 0) {  // at the ends of the tile's keys
         int r = w_row + l_row;
         asm volatile("" : "+v"(r));  // nothing of this is worth registers in the loop
         for (int u = 0; u < kPer; ++u, r += kWaveRows)
-          if (r >= valid)
+          if (r < lo || r >= hi)
             *reinterpret_cast<uint4 *>(lds_v[buf] + r * kRowBytes + l_chunk * 16) =
                 make_uint4(0u, 0u, 0u, 0u);
       }
     } else {
       store_k(buf);
-      store_rows(rv, lds_v[buf], TV{}, std::false_type{}, valid);
+      store_rows(rv, lds_v[buf], TV{}, std::false_type{}, lo, hi);
       if constexpr (!kWide) {
-        if (wave == 0) lds_vs[buf][lane] = fabsf(rvs) < INFINITY && lane < valid ? rvs : 0.f;
+        if (wave == 0) lds_vs[buf][lane] = fabsf(rvs) < INFINITY ? rvs : 0.f;
       }
     }
   };
@@ -854,7 +855,7 @@ void paged_prefill_kernel(PrefillParams p) {
     // a time through its own quarter of the K and V buffers, with no barrier; rows come
     // through registers, the next 32 keys' loads in flight during the math. (One wave on all
     // keys is bound by the time of a step: 31 sequences of one token on 1k-8k int8 keys beside
-    // a chunk of 1024, 32q/8kv HD 128, 179 us against the figure in launch_prefill_t.)
+    // a chunk of 1024, 32q/8kv HD 128, 179 us against 128.)
     constexpr int kFew = 32 / kWaveRows;
     constexpr int kFewPages = kUniform ? 2 : kFew;
     char *const own_k = lds_k[wave >> 1] + (wave & 1) * 32 * kRowBytes;
@@ -910,7 +911,7 @@ void paged_prefill_kernel(PrefillParams p) {
 #pragma unroll
       for (int u = 0; u < kFew; ++u) {
         const int r = u * kWaveRows + l_row;
-        const bool there = key0 + r < sq.len;
+        const bool there = key0 + r >= k_first && key0 + r < k_end;
         put(T{}, own_k + r * kRowBytes, fk[u], swizzle_k<HD>(r));
         const uint4 w = fv[u];
         put(TV{}, own_v + r * kRowBytes,
@@ -921,7 +922,7 @@ void paged_prefill_kernel(PrefillParams p) {
         if (lane < 32) {
           const bool whole = fabsf(fvs) < INFINITY;
           lds_ks[buf][r0 + lane] = whole ? fks : __builtin_nanf("");
-          lds_vs[buf][r0 + lane] = whole && key0 + lane < sq.len ? fvs : 0.f;
+          lds_vs[buf][r0 + lane] = whole ? fvs : 0.f;
         }
       }
       if (i + 1 < i1) {

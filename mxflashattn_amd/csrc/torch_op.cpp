@@ -75,6 +75,16 @@ at::Tensor workspace(const at::Device &device, void *stream, size_t bytes) {
   return it->second;
 }
 
+// Workspace of a call whose captures may be replayed beside each other: a graph gets memory of
+// its own pool, given back to the pool (for the graph's later calls) when the tensor goes.
+at::Tensor own_workspace(const at::Device &device, void *stream, size_t bytes) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing((hipStream_t)stream, &status) == hipSuccess &&
+      status != hipStreamCaptureStatusNone)
+    return at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(device));
+  return workspace(device, stream, bytes);
+}
+
 // First rows and lengths of a call on keys in consecutive rows: memory that no
 // other call or graph writes before the decode has read it (mxfa_package.h). A
 // graph gets memory of its own pool; eager calls of one stream, which follow each
@@ -616,7 +626,8 @@ py::object decode_tokens(const at::Tensor &q, const at::Tensor &k_cache, const a
     return py::none();
   void *stream = (void *)c10::hip::getCurrentHIPStream(device.index()).stream();
   at::Tensor ws_t;
-  if (ws_bytes) ws_t = workspace(device, stream, ws_bytes);
+  if (ws_bytes)
+    ws_t = rows ? own_workspace(device, stream, ws_bytes) : workspace(device, stream, ws_bytes);
   void *ws = ws_bytes ? ws_t.data_ptr() : nullptr;
   poison(stream, &out, ws_bytes ? &ws_t : nullptr);
   const int64_t esz = 2;
@@ -817,7 +828,7 @@ py::object prefill(const at::Tensor &q, const at::Tensor &k_cache, const at::Ten
     return py::none();
   void *stream = (void *)c10::hip::getCurrentHIPStream(device.index()).stream();
   at::Tensor ws_t;
-  if (ws_bytes) ws_t = workspace(device, stream, ws_bytes);
+  if (ws_bytes) ws_t = own_workspace(device, stream, ws_bytes);
   // A given output keeps the rows of no sequence.
   poison(stream, out_arg.has_value() ? nullptr : &out, ws_bytes ? &ws_t : nullptr);
   const int rc = mxfa_package_prefill_launch(

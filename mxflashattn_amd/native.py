@@ -54,6 +54,8 @@ FP8_DTYPE = torch.float8_e4m3fn
 # side's MXFA_PACKAGE_DTYPE_INT8 for int8).
 DTYPE_INT8 = 3
 ROW_DTYPES = {torch.float8_e4m3fn: DTYPE_FP8_E4M3, torch.int8: DTYPE_INT8}
+# A cache holds at most this many tokens of a sequence: a window of more hides nothing.
+MAX_WINDOW = 1 << 30
 
 # The reference's decode contract (vllm_plugin.py:220-261 hands other shapes
 # back); the guards that mirror the reference use these.
@@ -334,6 +336,14 @@ class _Workspace:
 
 
 WORKSPACE = _Workspace()
+
+
+def _own_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """Workspace of a call whose captures may be replayed beside each other: a graph gets
+    memory of its own pool instead of the stream's buffer."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return WORKSPACE.get(device, stream, nbytes)
 
 
 def retired_workspace_bytes() -> int:
@@ -830,7 +840,7 @@ def _paged_decode_rows(q, k_cache, v_cache, block_table, cache_seqlens, softmax_
     per_launch = tokens_per_launch(ql, gq, KERNEL_COLUMNS)
     stream = _stream_handle(q.device)
     ws_bytes = workspace_size(batch, hq * per_launch, hd, num_splits)
-    ws = WORKSPACE.get(q.device, stream, ws_bytes)
+    ws = _own_workspace(q.device, stream, max(ws_bytes, 1))
     _poison(out)
     q4, o4 = (q, out) if q.dim() == 4 else (q.unsqueeze(1), out.unsqueeze(1))
     cs = k_cache.stride()
@@ -839,8 +849,9 @@ def _paged_decode_rows(q, k_cache, v_cache, block_table, cache_seqlens, softmax_
         qc, oc = q4[:, first:end], o4[:, first:end]
         qs, os_ = qc.stride(), oc.stride()
         rc = library().mxfa_package_decode_rows_launch(
-            qc.data_ptr(), qs[0], qs[1], qs[2], end - first, int(causal), window_left,
-            _sinks_ptr(sinks, q), softcap, _sinks_ptr(alibi_slopes, q, "alibi_slopes"),
+            qc.data_ptr(), qs[0], qs[1], qs[2], end - first, int(causal),
+            min(int(window_left), MAX_WINDOW), _sinks_ptr(sinks, q), softcap,
+            _sinks_ptr(alibi_slopes, q, "alibi_slopes"),
             k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], *ks, *vs,
             block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), add,
             oc.data_ptr(), os_[0], os_[1], os_[2], ws.data_ptr(), ws_bytes, float(softmax_scale),
@@ -938,7 +949,7 @@ def paged_prefill(
     stream = _stream_handle(q.device)
     cus = num_cus(q.device.index or 0)
     ws_bytes = _prefill_workspace(batch, total, hq, hkv, hd, ps, block_table.shape[1], cus)
-    ws = WORKSPACE.get(q.device, stream, ws_bytes) if ws_bytes else None
+    ws = _own_workspace(q.device, stream, ws_bytes) if ws_bytes else None
     if final is None:
         _poison(out, ws)
     else:
@@ -949,8 +960,9 @@ def paged_prefill(
         k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2], *ks, *vs, k_one, v_one,
         block_table.data_ptr(), block_table.stride(0), cache_seqlens.data_ptr(), out.data_ptr(),
         out.stride(0), out.stride(1), ws.data_ptr() if ws is not None else 0, ws_bytes,
-        float(softmax_scale), int(bool(causal)), int(window_left), float(softcap),
-        _sinks_ptr(sinks, q), _sinks_ptr(alibi_slopes, q, "alibi_slopes"), batch, hq, hkv, hd, ps,
+        float(softmax_scale), int(bool(causal)), min(int(window_left), MAX_WINDOW),
+        float(softcap), _sinks_ptr(sinks, q), _sinks_ptr(alibi_slopes, q, "alibi_slopes"), batch,
+        hq, hkv, hd, ps,
         block_table.shape[1], pages, code,
         ROW_DTYPES.get(k_cache.dtype, code), cus, stream)
     _check(rc, "mxfa_package_prefill_launch")
@@ -1259,6 +1271,8 @@ def quantize_and_cache(
                     ("v_scale", v_scale)):
         if torch._debug_has_internal_overlap(t) == 1:
             raise ValueError(f"{name} must not have internally overlapping memory")
+    if key_cache.data_ptr() == value_cache.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr():
+        raise ValueError("the K and V caches and their scales must not share memory")
     key, value = _row_tensors(key, value)
     slots = slot_mapping.to(torch.int64).contiguous()
     n = key.shape[0]
@@ -1329,6 +1343,8 @@ def gather_cache(
             raise ValueError("dtype must be out's")
         if k.stride() != v.stride():
             raise UnsupportedConfig("out's tensors must share strides")
+        if total and k.data_ptr() == v.data_ptr():
+            raise ValueError("out's tensors must not share memory")
         dtype = k.dtype
     elif dtype is None:
         dtype = key_cache.dtype

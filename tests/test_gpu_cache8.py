@@ -302,6 +302,44 @@ def test_decode_of_rows_without_a_scale(device, codes):
         assert not bool(nan[1].any())
 
 
+@pytest.mark.parametrize("torch_op", [True, False], ids=["op", "ctypes"])
+def test_captured_decodes_side_by_side(device, monkeypatch, torch_op):
+    """Two graphs captured on one stream, replayed on two at once beside eager calls."""
+    monkeypatch.setattr(native, "USE_TORCH_OP", torch_op)
+    capture, other = torch.cuda.Stream(), torch.cuda.Stream()
+    calls = []
+    for seed in (3, 4):
+        p = make_paged([6000, 3000, 5000], 2, 128, BF16, 16, codes=INT8, seed=seed).to(device)
+        q = torch.randn(3, 8, 128, generator=torch.Generator().manual_seed(seed)).to(BF16)
+        calls.append((q.to(device), p))
+
+    def run(i):
+        q, p = calls[i]
+        return mx.paged_decode_split(q, p.kc, p.vc, p.table, p.lens, 0.1, num_splits=64,
+                                     k_scale=p.ks, v_scale=p.vs)
+
+    with torch.cuda.stream(capture):
+        want = [run(0).clone(), run(1).clone()]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=capture):
+            outs.append(run(i))
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+        with torch.cuda.stream(capture):
+            graphs[0].replay()
+            eager = run(1)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        assert torch.equal(eager, want[1])
+
+
 # ---------------------------------------------------------------------------
 # The run of them
 

@@ -176,6 +176,34 @@ def test_rows_without_a_scale_reach_only_tokens_that_see_them(device):
             assert not bool(nan[:, :2].any())
 
 
+@pytest.mark.parametrize("codes", [None, E4M3, INT8], ids=["16", "e4m3", "int8"])
+@pytest.mark.parametrize("new,window", [(1, 40), (9, 3), (9, 0), (70, 40), (1, 700), (200, 150)])
+def test_nan_ahead_of_the_window(device, codes, new, window):
+    """Keys ahead of every token's window may hold anything: their pages may be another's."""
+    length = 900
+    p = make_paged([length], 2, 64, BF16, 16, codes=codes)
+    q, cu = packed_q([new], 8, 64, BF16)
+    want, bound = expected(q, [new], p, 0.125, BF16, codes, window=window)
+    gone = torch.arange(length - new - window)
+    page, off = p.table[0].long()[gone // 16], gone % 16
+    for x, s in ((p.kc, p.ks), (p.vc, p.vs)):
+        if codes is None:
+            x[page, off] = float("nan")
+        else:
+            x.view(torch.uint8)[page, off] = 0x7F
+            s[page, :, off] = float("nan")
+    check(call(q, cu, p, 0.125, device, window=window), want, bound)
+
+
+def test_windows_past_the_positions(device):
+    """Windows of up to 2^31 - 1 and more hide nothing, with tokens ahead of the first key too."""
+    p = make_paged([30, 100], 2, 64, BF16, 16)
+    q, cu = packed_q([37, 20], 8, 64, BF16)
+    want, bound = expected(q, [37, 20], p, 0.125, BF16, None)
+    for window in (100, 2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1, 2 ** 32 + 3):
+        check(call(q, cu, p, 0.125, device, window=window), want, bound, f"window {window}")
+
+
 def test_scale_of_the_whole_cache(device):
     p = make_paged([150, 20], 2, 128, BF16, 16, fill=0.0)
     p = Paged(p.kc.to(E4M3), p.vc.to(E4M3), None, None, p.table, p.lens)
@@ -259,6 +287,44 @@ def test_streams_do_not_share_a_workspace(device):
         torch.cuda.synchronize()
         for out, (*_, (want, bound)) in zip(outs, cases):
             check(out, want, bound)
+
+
+@pytest.mark.parametrize("torch_op", [True, False], ids=["op", "ctypes"])
+def test_captured_calls_side_by_side(device, monkeypatch, torch_op):
+    """Two graphs captured on one stream, replayed on two at once beside eager calls on the
+    first: cut tiles' pieces of the one never meet the other's."""
+    monkeypatch.setattr(native, "USE_TORCH_OP", torch_op)
+    capture, other = torch.cuda.Stream(), torch.cuda.Stream()
+    calls = []
+    for seed in (3, 4):
+        p = make_paged([6000, 3000], 2, 128, BF16, 16, seed=seed).to(device)
+        q, cu = packed_q([8, 20], 8, 128, BF16, seed)
+        calls.append((q.to(device), p, cu.to(device)))
+
+    def run(i):
+        q, p, cu = calls[i]
+        return mx.paged_prefill(q, p.kc, p.vc, cu, p.table, p.lens, 0.1)
+
+    with torch.cuda.stream(capture):
+        want = [run(0).clone(), run(1).clone()]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], stream=capture):
+            outs.append(run(i))
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+        with torch.cuda.stream(capture):
+            graphs[0].replay()
+            eager = run(1)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+        assert torch.equal(eager, want[1])
 
 
 def test_pages_past_4_gib(device):
