@@ -641,11 +641,11 @@ void paged_prefill_kernel(PrefillParams p) {
 
   // K operand of the 32 keys in rows r0.. of buffer buf, dims 16 i ..; up to eight are read
   // ahead of their products.
-  constexpr int kReads = NQ < 8 ? NQ : 8;
+  constexpr int kReads = !kWide ? (NQ < 4 ? NQ : 4) : NQ < 8 ? NQ : 8;
   uint4 kf[kReads];
   // LDS addresses of the lane's operands, kept in registers where they fit (kUnroll): buffer
   // and row are then the reads' constant offsets.
-  constexpr bool kUnroll = kDirect && !kExtras;
+  constexpr bool kUnroll = kUniform && !kExtras && HD < 256;
   uint32_t k_at[NQ];
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
@@ -729,7 +729,7 @@ void paged_prefill_kernel(PrefillParams p) {
   float mr;  // the reference; 0 where no key is seen yet (the scores are -inf then)
   // 8-bit: V's scales of the lane's keys, all read ahead, or (fp16, where the split weights
   // take the registers) four keys ahead.
-  constexpr int kScales = kSplitP ? 2 : 4;
+  constexpr int kScales = 2;
   float4 vsc[kScales];
   auto read_vs = [&](int buf, int r0, int g) MXFA_INLINE {
     vsc[g % kScales] = *reinterpret_cast<const float4 *>(&lds_vs[buf][r0 + 8 * g + 4 * half]);
@@ -738,14 +738,14 @@ void paged_prefill_kernel(PrefillParams p) {
     mr = m == -INFINITY ? 0.f : m;
     if constexpr (!kWide) {
 #pragma unroll
-      for (int g = 0; g < kScales - (kSplitP ? 1 : 0); ++g) read_vs(buf, r0, g);
+      for (int g = 0; g < kScales - 1; ++g) read_vs(buf, r0, g);
     }
   };
   auto weigh = [&](auto ic, int buf, int r0, f32x16 &s) MXFA_INLINE {
     constexpr int i = decltype(ic)::value;
     s[i] = fast_exp2(__builtin_fmaf(s[i], cs, -mr));
     if constexpr (!kWide) {
-      if constexpr (kSplitP && i % 4 == 0 && i < 12) read_vs(buf, r0, i / 4 + 1);
+      if constexpr (i % 4 == 0 && i < 12) read_vs(buf, r0, i / 4 + 1);
       l += s[i];
       const float4 f = vsc[(i >> 2) % kScales];
       s[i] *= (i & 3) == 0 ? f.x : (i & 3) == 1 ? f.y : (i & 3) == 2 ? f.z : f.w;
