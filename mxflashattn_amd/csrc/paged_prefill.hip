@@ -170,6 +170,14 @@ int mxfa_package_prefill_launch(
   p.ps_log2 = __builtin_ctz((unsigned)page_size);
   p.max_len = (int)max_len;
   p.num_pages = num_pages;
+  // A window's keys, its tokens' windows together (and a tile's worth ahead of them).
+  const int64_t span = (int64_t)p.window_left + rows / gq + 1 + kPrefillKeys;
+  p.span = (int)(p.window_left < 0 || span > max_len ? max_len : span);
+  const auto mul = [](int d) {
+    return d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d);
+  };
+  p.hkv_mul = mul(kv_heads);
+  p.gq_mul = mul(gq);
   p.target = target;
   p.least = kLeastKeys;
   p.max_slots = 2 * target;

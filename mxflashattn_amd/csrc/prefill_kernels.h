@@ -77,6 +77,8 @@ struct PrefillParams {
   float softcap;       // 0: none
   int causal, window_left;
   int batch, rows_q, hkv, gq, ps_log2, max_len, num_pages;
+  uint32_t hkv_mul, gq_mul;  // div_by
+  int span;                  // keys that one row tile spans, at most
   int target;          // pieces per kv head that the keys are cut into (0: none)
   int least;           // fewest keys of a piece
   float *ws_o, *ws_lse;  // pieces: [slot][kv head][kRows][HD], [slot][kv head][kRows]
@@ -205,10 +207,35 @@ __device__ __forceinline__ void static_unroll(F &&f) {
   static_unroll_impl(f, std::make_integer_sequence<int, N>{});
 }
 
+// x / d for 0 <= x < 2^31 and 1 <= d < 2^16 by m = ceil(2^32 / d) (0 for d = 1): x m / 2^32
+// passes x / d by less than a half, so the quotient is one too many at most.
+__device__ __forceinline__ int div_by(int x, int d, uint32_t m) {
+  const uint32_t q = m ? __umulhi((uint32_t)x, m) : (uint32_t)x;
+  return (int)(q - (q * (uint32_t)d > (uint32_t)x ? 1u : 0u));
+}
+
+// A wave's fold of values with identity 0, in every lane.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_fold(T x, F f) {
+  const auto with = [&](int y) { x = f(x, __builtin_bit_cast(T, y)); };
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kDppRowShr0 + 1, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kDppRowShr0 + 2, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kDppRowShr0 + 4, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kDppRowShr0 + 8, 0xf, 0xf, true));
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kDppRowBcast15, 0xa, 0xf, false));
+  with(__builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kDppRowBcast31, 0xc, 0xf, false));
+  return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  return wave_fold(x, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ int wave_sum(int x) {
+  return wave_fold(x, [](int a, int b) { return a + b; });
+}
+
 // What one sequence asks for: its query rows and keys, held to those that exist.
 struct PrefillSeq {
-  int start, n, len, tiles, span;
-  bool few;  // at most 32 rows in a call whose tiles may be cut: all waves on one row tile
+  int start, n, len;
 };
 
 __device__ __forceinline__ PrefillSeq prefill_seq(const PrefillParams &p, int b) {
@@ -217,22 +244,21 @@ __device__ __forceinline__ PrefillSeq prefill_seq(const PrefillParams &p, int b)
   const int end = min(max(p.cu[b + 1], s.start), p.rows_q);
   s.n = end - s.start;
   s.len = min(max(p.seqlens[b], 0), p.max_len);
-  const int64_t rows = (int64_t)s.n * p.gq;
-  s.few = p.target > 0 && rows <= 32;
-  s.tiles = (int)((rows + kPrefillRows - 1) / kPrefillRows);
-  // Keys that one row tile spans, at most: with a window its tokens' windows together.
-  s.span = p.window_left < 0 ? s.len
-                             : (int)min((int64_t)s.len, (int64_t)p.window_left +
-                                                            kPrefillRows / p.gq + 1 + kPrefillKeys);
   return s;
 }
-
-// What a key of a row tile costs: four waves on their own keys take half of a tile's time.
-__device__ __forceinline__ int prefill_cost(const PrefillSeq &q) {
-  return q.few ? (q.span + 1) / 2 : q.span;
+__device__ __forceinline__ int prefill_tiles(const PrefillParams &p, const PrefillSeq &q) {
+  return (int)(((int64_t)q.n * p.gq + kPrefillRows - 1) / kPrefillRows);
 }
-__device__ __forceinline__ int prefill_pieces(const PrefillSeq &q, int most) {
-  const int cost = prefill_cost(q);
+// At most 32 rows in a call whose tiles may be cut: all waves on one row tile.
+__device__ __forceinline__ bool prefill_few(const PrefillParams &p, const PrefillSeq &q) {
+  return p.target > 0 && (int64_t)q.n * p.gq <= 32;
+}
+// What a row tile costs, in keys: four waves on their own keys take half of a tile's time.
+__device__ __forceinline__ int prefill_cost(const PrefillParams &p, const PrefillSeq &q) {
+  const int span = min(q.len, p.span);
+  return prefill_few(p, q) ? (span + 1) / 2 : span;
+}
+__device__ __forceinline__ int prefill_pieces(int cost, int most) {
   return cost > most ? (cost + most - 1) / most : 1;
 }
 // Keys (at their cost) of a piece: W / target, a little more so that 32-bit sums of W keep
@@ -244,19 +270,14 @@ __device__ __forceinline__ int prefill_most(const PrefillParams &p, float work) 
 
 struct PrefillItem {
   int b, tile, piece, pieces, slot;
+  PrefillSeq seq;
 };
 
 struct PrefillScan {
   float work[kPrefillWaves];
   int items[kPrefillWaves], slots[kPrefillWaves];
-  PrefillItem item;
+  int b, tile, piece, pieces, slot;
 };
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-  return x;
-}
 
 // The row tile and piece of item `index`; b = -1 past the last.
 //
@@ -270,31 +291,32 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (p.batch <= 64) {
     const PrefillSeq q = prefill_seq(p, min(lane, p.batch - 1));
-    const int tiles = lane < p.batch ? q.tiles : 0;
-    const int most =
-        p.target > 0 ? prefill_most(p, wave_sum((float)tiles * (float)prefill_cost(q))) : 0x7fffffff;
-    const int pieces = prefill_pieces(q, most);
-    const auto total = [](int x) { return __builtin_amdgcn_readlane(wave_scan_incl(x), 63); };
+    const int tiles = lane < p.batch ? prefill_tiles(p, q) : 0;
+    int pieces = 1;
+    if (p.target > 0) {
+      const int cost = prefill_cost(p, q);
+      const int most = prefill_most(p, wave_sum((float)tiles * (float)cost));
+      if (__builtin_amdgcn_ballot_w64(cost > most) != 0) pieces = prefill_pieces(cost, most);
+    }
     const int cut = pieces > 1 ? tiles * pieces : 0;
     const int slots = wave_scan_incl(cut);
     if (tell && p.target > 0 && threadIdx.x == 0)
       *p.ws_total = min(__builtin_amdgcn_readlane(slots, 63), p.max_slots);
-    // The round: the largest d whose items of earlier rounds are at most `index`.
+    if (index >= wave_sum(tiles * pieces)) return {-1, 0, 0, 1, 0, q};
+    // The round: the largest d whose items of earlier rounds are at most `index`, 64
+    // candidates at a time.
     int lo = 0, before = 0;
-    int hi = tiles;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) hi = max(hi, __shfl_xor(hi, d));
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    if (index >= total(tiles * pieces)) return {-1, 0, 0, 1, 0};
+    int hi = wave_fold(tiles, [](int a, int b) { return max(a, b); });
     while (hi - lo > 1) {  // items before round lo <= index < items before round hi
-      const int mid = lo + ((hi - lo) >> 1);
-      const int items = total(pieces * min(tiles, mid));
-      if (items <= index) {
-        lo = mid;
-        before = items;
-      } else {
-        hi = mid;
-      }
+      const int step = (hi - lo + 63) >> 6, d = lo + lane * step;
+      int items = 0;
+#pragma unroll 4
+      for (int b = 0; b < p.batch; ++b)
+        items += __builtin_amdgcn_readlane(pieces, b) * min(__builtin_amdgcn_readlane(tiles, b), d);
+      const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(items <= index)) - 1;
+      before = __builtin_amdgcn_readlane(items, at);
+      lo += at * step;
+      hi = min(hi, lo + step);
     }
     const int here = tiles > lo ? pieces : 0;
     const int upto = wave_scan_incl(here);
@@ -303,7 +325,7 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
     const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
     const int piece = index - before - (of(upto) - of(here));
     return {b, of(tiles) - 1 - lo, piece, of(pieces),
-            of(slots) - of(cut) + lo * of(pieces) + piece};
+            of(slots) - of(cut) + lo * of(pieces) + piece, {of(q.start), of(q.n), of(q.len)}};
   }
   const int per = (p.batch + kPrefillWaves * 64 - 1) / (kPrefillWaves * 64);
   const int b0 = threadIdx.x * per, b1 = min(b0 + per, p.batch);
@@ -312,7 +334,7 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
     float work = 0.f;
     for (int b = b0; b < b1; ++b) {
       const PrefillSeq q = prefill_seq(p, b);
-      work += (float)q.tiles * (float)prefill_cost(q);
+      work += (float)prefill_tiles(p, q) * (float)prefill_cost(p, q);
     }
     work = wave_sum(work);
     if (lane == 0) s.work[wave] = work;
@@ -325,16 +347,17 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
   int items = 0, slots = 0;
   for (int b = b0; b < b1; ++b) {
     const PrefillSeq q = prefill_seq(p, b);
-    const int pieces = prefill_pieces(q, most);
-    items += q.tiles * pieces;
-    slots += pieces > 1 ? q.tiles * pieces : 0;
+    const int pieces = prefill_pieces(prefill_cost(p, q), most);
+    const int here = prefill_tiles(p, q) * pieces;
+    items += here;
+    slots += pieces > 1 ? here : 0;
   }
   const int items_in = wave_scan_incl(items), slots_in = wave_scan_incl(slots);
   if (lane == 63) {
     s.items[wave] = items_in;
     s.slots[wave] = slots_in;
   }
-  if (threadIdx.x == 0) s.item.b = -1;
+  if (threadIdx.x == 0) s.b = -1;
   __syncthreads();
   int items_at = items_in - items, slots_at = slots_in - slots, slots_all = 0;
 #pragma unroll
@@ -346,15 +369,15 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
   if (index >= items_at && index < items_at + items) {
     for (int b = b0; b < b1; ++b) {
       const PrefillSeq q = prefill_seq(p, b);
-      const int pieces = prefill_pieces(q, most);
-      const int here = q.tiles * pieces;
+      const int pieces = prefill_pieces(prefill_cost(p, q), most);
+      const int tiles = prefill_tiles(p, q), here = tiles * pieces;
       if (index < items_at + here) {
         const int local = index - items_at;
-        s.item.b = b;
-        s.item.tile = q.tiles - 1 - local / pieces;
-        s.item.piece = local % pieces;
-        s.item.pieces = pieces;
-        s.item.slot = slots_at + local;
+        s.b = b;
+        s.tile = tiles - 1 - local / pieces;
+        s.piece = local % pieces;
+        s.pieces = pieces;
+        s.slot = slots_at + local;
         break;
       }
       items_at += here;
@@ -365,8 +388,9 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
   __syncthreads();
   // The same in every lane: scalars, and so is what follows from them.
   const auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  return {uniform(s.item.b), uniform(s.item.tile), uniform(s.item.piece), uniform(s.item.pieces),
-          uniform(s.item.slot)};
+  const int b = uniform(s.b);
+  return {b, uniform(s.tile), uniform(s.piece), uniform(s.pieces), uniform(s.slot),
+          prefill_seq(p, max(b, 0))};
 }
 
 // One row tile (and piece of its keys) of one kv head.
@@ -400,38 +424,49 @@ void paged_prefill_kernel(PrefillParams p) {
   __shared__ PrefillScan scan;
   __shared__ float few_m[kPrefillWaves][32], few_l[kPrefillWaves][32];
 
-  const int kvh = blockIdx.x % p.hkv;
-  const PrefillItem it = prefill_find(p, blockIdx.x / p.hkv, scan, blockIdx.x == 0);
+  const int item = div_by(blockIdx.x, p.hkv, p.hkv_mul), kvh = blockIdx.x - item * p.hkv;
+  const PrefillItem it = prefill_find(p, item, scan, blockIdx.x == 0);
   if (it.b < 0) return;
   if (it.pieces > 1 && it.slot >= p.max_slots) return;
-  const PrefillSeq sq = prefill_seq(p, it.b);
+  const PrefillSeq sq = it.seq;
+  const bool few = prefill_few(p, sq);
   // The wave's number and what follows from it are scalars.
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int gq = p.gq;
   const int rows = sq.n * gq;  // of the sequence, per kv head
   const int first_pos = sq.len - sq.n;
+  // The tile's first row: token t_first, head r_first; row r of the tile is then
+  // token_of(r_first + r) tokens on (numbers below 2^8, divided exactly).
+  const int t_first = div_by(it.tile * kRows, gq, p.gq_mul);
+  const int r_first = it.tile * kRows - t_first * gq;
+  const uint32_t small = (p.gq_mul >> 16) + 1;  // 2^16 / gq, or a little more
+  const auto token_of = [&](int r) { return gq == 1 ? r : (int)((uint32_t)r * small >> 16); };
 
   // Keys that some row of the tile sees, [k_first, k_end), then tiles of KT of them, then the
   // piece's.
-  const int t_first = it.tile * kRows / gq;
-  const int t_last = min(sq.n - 1, (it.tile * kRows + kRows - 1) / gq);
+  const int t_last = min(sq.n - 1, t_first + token_of(r_first + kRows - 1));
   const int k_end = max(0, p.causal ? min(sq.len, first_pos + t_last + 1) : sq.len);
   const int k_first = p.window_left >= 0 ? max(0, first_pos + t_first - p.window_left) : 0;
   const int k_begin = k_first / KT * KT;
   const int all = k_end > k_begin ? (k_end - k_begin + KT - 1) / KT : 0;
-  const int j0 = (int)((int64_t)all * it.piece / it.pieces);
-  const int j1 = (int)((int64_t)all * (it.piece + 1) / it.pieces);
+  int j0 = 0, j1 = all;
+  if (it.pieces > 1) {
+    j0 = (int)((int64_t)all * it.piece / it.pieces);
+    j1 = (int)((int64_t)all * (it.piece + 1) / it.pieces);
+  }
 
   // This lane's row, and the wave's rows.
-  const int row_w = sq.few ? 0 : it.tile * kRows + wave * 32;
-  const int row = row_w + col;
-  const bool live = row < rows;
-  const int tok = min(row, rows - 1) / gq, head = min(row, rows - 1) % gq;
+  const int in_tile = few ? 0 : wave * 32;
+  const int row_w = it.tile * kRows + in_tile;
+  const bool live = row_w + col < rows;
+  const int ahead = token_of(r_first + in_tile + col);  // tokens from t_first on
+  const int tok = live ? t_first + ahead : sq.n - 1;
+  const int head = live ? r_first + in_tile + col - ahead * gq : gq - 1;
   const int pos = first_pos + tok;
   // Keys that all of the wave's rows see, [all_from, all_to], and the last that any does.
-  const int pos_lo = first_pos + row_w / gq;
-  const int pos_hi = first_pos + min(row_w + 31, rows - 1) / gq;
+  const int pos_lo = first_pos + t_first + token_of(r_first + in_tile);
+  const int pos_hi = first_pos + min(t_first + token_of(r_first + in_tile + 31), sq.n - 1);
   const int all_to = p.causal ? min(pos_lo, sq.len - 1) : sq.len - 1;
   const int all_from = p.window_left < 0 ? 0 : pos_hi - p.window_left;
   const int any_to = row_w >= rows ? -1
@@ -451,14 +486,14 @@ void paged_prefill_kernel(PrefillParams p) {
   // reference. c > 0: a negative scale's sign goes to q, and a scale of zero zeroes q.
   float c = p.scale * kPrefillLog2e;
   if (!kWide && p.k_scale) c *= p.k_scale[0];
-  {
-    const uint32_t keep = c == 0.f ? 0u : 0xffffffffu, flip = c < 0.f ? 0x80008000u : 0u;
+  const uint32_t keep = c == 0.f ? 0u : 0xffffffffu, flip = c < 0.f ? 0x80008000u : 0u;
+  c = c == 0.f ? 1.f : fabsf(c);
+  const auto sign_q = [&]() MXFA_INLINE {  // (once the first keys' loads are out)
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
       qf[i] = make_uint4((qf[i].x ^ flip) & keep, (qf[i].y ^ flip) & keep,
                          (qf[i].z ^ flip) & keep, (qf[i].w ^ flip) & keep);
-    c = c == 0.f ? 1.f : fabsf(c);
-  }
+  };
   const float cs = kExtras ? 1.f : c;  // what is left to multiply scores by at the exponent
   const float v_scale = !kWide && p.v_scale ? p.v_scale[0] : 1.f;
   const bool capped = kExtras && p.softcap > 0.f;
@@ -482,8 +517,11 @@ void paged_prefill_kernel(PrefillParams p) {
   // the first of tile j + 1.
   constexpr int kAhead = KT / 2;
   float rks = 0.f, rvk = 0.f, rvs = 0.f;  // 8-bit: scales of stage row `lane` (vs at K's key too)
-  // Page ids of the rows to load next: one for the wave's rows of K and of V (kUniform), else
-  // one for each of this lane's.
+  // Page ids of the rows to load next: one for the wave's rows of K and of V (kUniform: K's in
+  // the lower half's lanes of pg_k, V's in the upper's), else one for each of this lane's.
+  // They are vector loads, a tile ahead, which the wait for that tile's rows covers: a scalar
+  // load in flight makes every wait for an LDS read wait for it too (64 keys of a wave alone
+  // on its SIMD: 3460 cycles, 2260 without the loads).
   constexpr int kPages = kUniform ? 1 : kPer;
   int pg_k[kPages], pg_v[kPages], pg_ks = 0, pg_vs = 0;
 
@@ -492,14 +530,12 @@ void paged_prefill_kernel(PrefillParams p) {
   auto page_at = [&](int key) MXFA_INLINE { return min(max(key, 0) >> p.ps_log2, last_page); };
   auto find_pages = [&](int j) MXFA_INLINE {
     const int key0 = k_begin + j * KT;
+    if constexpr (kUniform) {
+      pg_k[0] = bt[page_at(key0 + w_row + (half ? 0 : kAhead))];
+    } else {
 #pragma unroll
-    for (int u = 0; u < kPages; ++u) {
-      const int r = w_row + (kUniform ? 0 : u * kWaveRows + l_row);
-      if constexpr (kUniform) {
-        const auto table = (const __attribute__((address_space(4))) int32_t *)bt;
-        pg_k[u] = table[page_at(key0 + kAhead + r)];
-        pg_v[u] = table[page_at(key0 + r)];
-      } else {
+      for (int u = 0; u < kPages; ++u) {
+        const int r = w_row + u * kWaveRows + l_row;
         pg_k[u] = bt[page_at(key0 + kAhead + r)];
         pg_v[u] = bt[page_at(key0 + r)];
       }
@@ -522,7 +558,8 @@ void paged_prefill_kernel(PrefillParams p) {
   auto load_rows = [&](const char *side, int key0, const int (&pg)[kPages], auto is_k, char *lds,
                        uint4 (&reg)[kDirect ? 1 : kPer]) MXFA_INLINE {
     if constexpr (kUniform) {
-      const char *src = uniform_pointer(side + row_off(key0 + w_row, pg[0]));
+      const int page = __builtin_amdgcn_readlane(pg[0], decltype(is_k)::value ? 0 : 32);
+      const char *src = uniform_pointer(side + row_off(key0 + w_row, page));
       uint32_t at = lds_offset(lds) + w_row * kRowBytes;
       static_unroll<kPer>([&](auto uc) {
         constexpr int u = decltype(uc)::value;
@@ -546,21 +583,24 @@ void paged_prefill_kernel(PrefillParams p) {
             side + row_off(key0 + w_row + u * kWaveRows + l_row, pg[u]) + l_chunk * 16);
     }
   };
-  auto load_k_scales = [&](int key0) MXFA_INLINE {
+  auto load_k_scales = [&](int key0, int id) MXFA_INLINE {
     if constexpr (!kWide) {
       if (wave == 0) {
         const int off = (key0 + lane) & ps_mask;
-        const int64_t page = min(max(pg_ks, 0), p.num_pages - 1);
+        const int64_t page = min(max(id, 0), p.num_pages - 1);
         rks = p.ks ? p.ks[page * p.ks_sp + (int64_t)kvh * p.ks_sh + off] : 1.f;
         rvk = p.vs ? p.vs[page * p.vs_sp + (int64_t)kvh * p.vs_sh + off] : 1.f;
       }
     }
   };
-  auto load_tile = [&](int j, int buf) MXFA_INLINE {
+  auto load_k = [&](int j, int buf) MXFA_INLINE {
+    const int key0 = k_begin + j * KT + kAhead;
+    load_rows(p.k, key0, pg_k, std::true_type{}, lds_k[buf], rk);
+    load_k_scales(key0, pg_ks);
+  };
+  auto load_v = [&](int j, int buf) MXFA_INLINE {
     const int key0 = k_begin + j * KT;
-    load_rows(p.k, key0 + kAhead, pg_k, std::true_type{}, lds_k[buf], rk);
-    load_rows(p.v, key0, pg_v, std::false_type{}, lds_v[buf], rv);
-    load_k_scales(key0 + kAhead);
+    load_rows(p.v, key0, kUniform ? pg_k : pg_v, std::false_type{}, lds_v[buf], rv);
     if constexpr (!kWide) {
       if (wave == 0) {
         const int64_t page = min(max(pg_vs, 0), p.num_pages - 1);
@@ -568,6 +608,10 @@ void paged_prefill_kernel(PrefillParams p) {
                    : 1.f;
       }
     }
+  };
+  auto load_tile = [&](int j, int buf) MXFA_INLINE {
+    load_k(j, buf);
+    load_v(j, buf);
   };
   // 16 loaded bytes of a row into its LDS row, an 8-bit cache's widened.
   auto put = [&](auto type, char *dst, const uint4 &w, int sw) MXFA_INLINE {
@@ -645,7 +689,7 @@ void paged_prefill_kernel(PrefillParams p) {
   uint4 kf[kReads];
   // LDS addresses of the lane's operands, kept in registers where they fit (kUnroll): buffer
   // and row are then the reads' constant offsets.
-  constexpr bool kUnroll = kUniform && !kExtras && HD < 256;
+  constexpr bool kUnroll = kUniform && !kExtras && HD < 256 && !(kSplitP && HD == 128);
   uint32_t k_at[NQ];
 #pragma unroll
   for (int i = 0; i < NQ; ++i) {
@@ -850,14 +894,14 @@ void paged_prefill_kernel(PrefillParams p) {
       advance(buf, r0, cur, nxt);  // (past the last keys, products that nobody looks at)
     }
   };
-  if (sq.few) {
+  if (few) {
     // Few rows: the four waves share them and each takes a quarter of the piece's keys, 32 at
     // a time through its own quarter of the K and V buffers, with no barrier; rows come
     // through registers, the next 32 keys' loads in flight during the math. (One wave on all
     // keys is bound by the time of a step: 31 sequences of one token on 1k-8k int8 keys beside
     // a chunk of 1024, 32q/8kv HD 128, 179 us against 128.)
     constexpr int kFew = 32 / kWaveRows;
-    constexpr int kFewPages = kUniform ? 2 : kFew;
+    constexpr int kFewPages = kUniform ? 1 : kFew;  // (kUniform: of 16 rows, in each half)
     char *const own_k = lds_k[wave >> 1] + (wave & 1) * 32 * kRowBytes;
     char *const own_v = lds_v[wave >> 1] + (wave & 1) * 32 * kRowBytes;
     const int buf = wave >> 1, r0 = (wave & 1) * 32;
@@ -872,8 +916,7 @@ void paged_prefill_kernel(PrefillParams p) {
 #pragma unroll
       for (int u = 0; u < kFewPages; ++u) {
         if constexpr (kUniform)
-          pages[u] =
-              ((const __attribute__((address_space(4))) int32_t *)bt)[page_at(key0 + 16 * u)];
+          pages[u] = bt[page_at(key0 + 16 * half)];
         else
           pages[u] = bt[page_at(key0 + u * kWaveRows + l_row)];
       }
@@ -886,7 +929,7 @@ void paged_prefill_kernel(PrefillParams p) {
         const int r = u * kWaveRows;
         int64_t off;
         if constexpr (kUniform)
-          off = row_off(key0 + r, pages[r >> 4]) + lane_off;
+          off = row_off(key0 + r, __builtin_amdgcn_readlane(pages[0], r < 16 ? 0 : 32)) + lane_off;
         else
           off = row_off(key0 + r + l_row, pages[u]);
         off += l_chunk * 16;
@@ -906,6 +949,7 @@ void paged_prefill_kernel(PrefillParams p) {
       few_load(i);
       few_pages(i + 1);
     }
+    sign_q();
     for (; i < i1; ++i) {
       const int key0 = base + 32 * i;
 #pragma unroll
@@ -949,13 +993,19 @@ void paged_prefill_kernel(PrefillParams p) {
     }
   } else if (j0 < j1) {
     f32x16 sa, sb;
-    // K's stage before the first holds the first 32 keys.
+    // K's stage before the first holds the first 32 keys. Loads go out as their pages come.
     find_pages(j0 - 1);
-    load_rows(p.k, k_begin + j0 * KT - kAhead, pg_k, std::true_type{}, lds_k[1], rk);
-    load_k_scales(k_begin + j0 * KT - kAhead);
+    int pg_0[kPages];
+#pragma unroll
+    for (int u = 0; u < kPages; ++u) pg_0[u] = pg_k[u];
+    const int pg_s0 = pg_ks;
     find_pages(j0);
+    load_rows(p.k, k_begin + j0 * KT - kAhead, pg_0, std::true_type{}, lds_k[1], rk);
+    load_k_scales(k_begin + j0 * KT - kAhead, pg_s0);
+    load_v(j0, 0);
     if constexpr (!kDirect) store_k(1);
-    load_tile(j0, 0);
+    load_k(j0, 0);
+    sign_q();
     find_pages(j0 + 1);
     if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -991,7 +1041,7 @@ void paged_prefill_kernel(PrefillParams p) {
   const auto lw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false,
                                                    false);
   l = __uint_as_float(lw[0]) + __uint_as_float(lw[1]);
-  if (sq.few) {
+  if (few) {
     // The four waves' rows: references and sums, then the accumulators as [4 dims][row] through
     // the K (waves 0, 1) and V (2, 3) buffers; thread (part, row) then joins HD / 8 dims of a
     // row in wave order.
@@ -1031,11 +1081,11 @@ void paged_prefill_kernel(PrefillParams p) {
       inv = ll == 0.f ? 0.f : v_scale / ll;
     } else {
       float den = ll;
-      if (p.sinks) den += fast_exp2(p.sinks[kvh * gq + r % gq] * kPrefillLog2e - mm);
+      if (p.sinks) den += fast_exp2(p.sinks[kvh * gq + r - token_of(r) * gq] * kPrefillLog2e - mm);
       inv = ll == 0.f ? 0.f : v_scale / den;
     }
-    char *const dst = p.out + (int64_t)(sq.start + r / gq) * p.o_st +
-                      (int64_t)(kvh * gq + r % gq) * p.o_sh;
+    char *const dst = p.out + (int64_t)(sq.start + token_of(r)) * p.o_st +
+                      (int64_t)(kvh * gq + r - token_of(r) * gq) * p.o_sh;
 #pragma unroll
     for (int cc = 0; cc < HD / 32; ++cc) {
       const int chunk = part * (HD / 32) + cc;
