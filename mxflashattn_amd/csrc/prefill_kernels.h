@@ -197,6 +197,18 @@ __device__ __forceinline__ void load_to_lds(const char *base, uint32_t off, uint
                : "memory");
 }
 
+// The same where `on` is ~0; no load where it is 0. (A branch amid the products makes the
+// compiler copy their accumulators.)
+__device__ __forceinline__ void load_to_lds_if(const char *base, uint32_t off, uint32_t lds,
+                                               uint64_t on) {
+  uint64_t all;
+  asm volatile("s_mov_b32 m0, %1\n\ts_and_saveexec_b64 %0, %4\n\t"
+               "global_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0"
+               : "=&s"(all)
+               : "s"(lds), "v"(off), "s"(base), "s"(on)
+               : "memory", "scc");
+}
+
 // f(std::integral_constant<int, I>) for I = 0 .. N-1, unrolled at compile time.
 template <typename F, int... I>
 __device__ __forceinline__ void static_unroll_impl(F &&f, std::integer_sequence<int, I...>) {
@@ -247,11 +259,11 @@ __device__ __forceinline__ PrefillSeq prefill_seq(const PrefillParams &p, int b)
   return s;
 }
 __device__ __forceinline__ int prefill_tiles(const PrefillParams &p, const PrefillSeq &q) {
-  return (int)(((int64_t)q.n * p.gq + kPrefillRows - 1) / kPrefillRows);
+  return (int)((uint32_t)(q.n * p.gq + kPrefillRows - 1) / kPrefillRows);  // (a call's rows: int)
 }
 // At most 32 rows in a call whose tiles may be cut: all waves on one row tile.
 __device__ __forceinline__ bool prefill_few(const PrefillParams &p, const PrefillSeq &q) {
-  return p.target > 0 && (int64_t)q.n * p.gq <= 32;
+  return p.target > 0 && q.n * p.gq <= 32;
 }
 // What a row tile costs, in keys: four waves on their own keys take half of a tile's time.
 __device__ __forceinline__ int prefill_cost(const PrefillParams &p, const PrefillSeq &q) {
@@ -302,7 +314,7 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
     const int slots = wave_scan_incl(cut);
     if (tell && p.target > 0 && threadIdx.x == 0)
       *p.ws_total = min(__builtin_amdgcn_readlane(slots, 63), p.max_slots);
-    if (index >= wave_sum(tiles * pieces)) return {-1, 0, 0, 1, 0, q};
+    if (index >= wave_sum(tiles * pieces)) return {-1, 0, 0, 1, 0, {0, 0, 0}};
     // The round: the largest d whose items of earlier rounds are at most `index`, 64
     // candidates at a time.
     int lo = 0, before = 0;
@@ -389,8 +401,9 @@ __device__ __forceinline__ PrefillItem prefill_find(const PrefillParams &p, int 
   // The same in every lane: scalars, and so is what follows from them.
   const auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const int b = uniform(s.b);
+  const PrefillSeq q = prefill_seq(p, max(b, 0));
   return {b, uniform(s.tile), uniform(s.piece), uniform(s.pieces), uniform(s.slot),
-          prefill_seq(p, max(b, 0))};
+          {uniform(q.start), uniform(q.n), uniform(q.len)}};
 }
 
 // One row tile (and piece of its keys) of one kv head.
@@ -846,7 +859,9 @@ void paged_prefill_kernel(PrefillParams p) {
     if constexpr (!kExtras) top = largest(s);
   };
   // The weights of cur's keys and their part of the output, and nxt's scores.
-  auto advance = [&](int buf, int r0, f32x16 &cur, f32x16 &nxt) MXFA_INLINE {
+  // between(slot): work after the slot-th product of NQ + 2 ND.
+  const auto nothing = [](auto) MXFA_INLINE {};
+  auto advance = [&](int buf, int r0, f32x16 &cur, f32x16 &nxt, auto between) MXFA_INLINE {
 #pragma unroll
     for (int i = 0; i < kReads; ++i) read_k(buf, r0, i);
     weigh_start(buf, r0);
@@ -867,33 +882,60 @@ void paged_prefill_kernel(PrefillParams p) {
           vf[d] = read_v(buf, r0, d);
         });
       }
+      between(ic);
       __builtin_amdgcn_sched_barrier(0);
     });
     uint4 vn[ND];
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const uint4 w = make_uint4(pf[4 * st], pf[4 * st + 1], pf[4 * st + 2], pf[4 * st + 3]);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const uint4 a = st ? vn[d] : vf[d];
-        o[d] = Prod32<TV>::run(a, w, o[d]);
-        if constexpr (kSplitP)
-          o[d] = Prod32<TV>::run(
-              a, make_uint4(pl[4 * st], pl[4 * st + 1], pl[4 * st + 2], pl[4 * st + 3]), o[d]);
-        if (st == 0) vn[d] = read_v(buf, r0 + 16, d);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (st == 0) scale_scores(buf, r0, nxt);
-    }
+    static_unroll<2 * ND>([&](auto ic) {
+      constexpr int st = decltype(ic)::value / ND, d = decltype(ic)::value % ND;
+      const uint4 a = st ? vn[d] : vf[d];
+      o[d] = Prod32<TV>::run(
+          a, make_uint4(pf[4 * st], pf[4 * st + 1], pf[4 * st + 2], pf[4 * st + 3]), o[d]);
+      if constexpr (kSplitP)
+        o[d] = Prod32<TV>::run(
+            a, make_uint4(pl[4 * st], pl[4 * st + 1], pl[4 * st + 2], pl[4 * st + 3]), o[d]);
+      if constexpr (st == 0) vn[d] = read_v(buf, r0 + 16, d);
+      between(std::integral_constant<int, NQ + decltype(ic)::value>{});
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (st == 0 && d == ND - 1) scale_scores(buf, r0, nxt);
+    });
     if constexpr (!kExtras) top = largest(nxt);
   };
-  auto step = [&](int key0, int buf, int r0, f32x16 &cur, f32x16 &nxt) MXFA_INLINE {
+  auto step = [&](int key0, int buf, int r0, f32x16 &cur, f32x16 &nxt, auto between) MXFA_INLINE {
     if (key0 <= any_to) {  // some row of the wave sees some of the 32 keys
       limit(key0, cur, top);
       refer(top);
-      advance(buf, r0, cur, nxt);  // (past the last keys, products that nobody looks at)
+      // (past the last keys, products that nobody looks at)
+      advance(buf, r0, cur, nxt, between);
     }
   };
+  // Rows straight to LDS: a wave's 2 kPer loads of the next tile go out one by one among the
+  // first step's products. (All at once they hold the wave up: the CU takes 64 bytes a clock,
+  // 512 clocks for a tile of the four waves.)
+  auto spread_load = [&](int j, int buf, bool more) MXFA_INLINE {
+    const int key0 = k_begin + j * KT + w_row;
+    const int page_k = __builtin_amdgcn_readlane(pg_k[0], 0);
+    const int page_v = __builtin_amdgcn_readlane(pg_k[0], 32);
+    const char *const src_k = uniform_pointer(p.k + row_off(key0 + kAhead, page_k));
+    const char *const src_v = uniform_pointer(p.v + row_off(key0, page_v));
+    const uint32_t to_k = lds_offset(lds_k[buf]) + w_row * kRowBytes;
+    const uint32_t to_v = lds_offset(lds_v[buf]) + w_row * kRowBytes;
+    const uint32_t half_on = __builtin_amdgcn_readfirstlane(more ? 0xffffffffu : 0u);
+    const uint64_t on = (uint64_t)half_on << 32 | half_on;
+    return [=](auto slot) MXFA_INLINE {
+      constexpr int s = decltype(slot)::value;
+      constexpr bool is_k = s < NQ;
+      constexpr int apart = is_k ? NQ / kPer : 2 * ND / kPer, i = is_k ? s : s - NQ;
+      if constexpr (i % apart == 0 && i / apart < kPer) {
+        constexpr int u = i / apart;
+        const int r = u * kWaveRows + l_row;
+        const int from = is_k ? l_chunk ^ swizzle_k<HD>(r) : l_chunk ^ swizzle_v<HD>(r);
+        load_to_lds_if((is_k ? src_k : src_v) + u * kWaveRows * st, lane_off + from * 16,
+                       (is_k ? to_k : to_v) + u * kWaveRows * kRowBytes, on);
+      }
+    };
+  };
+  if constexpr (!kDirect) sign_q();  // (later, the unsigned q would take registers too)
   if (few) {
     // Few rows: the four waves share them and each takes a quarter of the piece's keys, 32 at
     // a time through its own quarter of the K and V buffers, with no barrier; rows come
@@ -949,7 +991,7 @@ void paged_prefill_kernel(PrefillParams p) {
       few_load(i);
       few_pages(i + 1);
     }
-    sign_q();
+    if constexpr (kDirect) sign_q();
     for (; i < i1; ++i) {
       const int key0 = base + 32 * i;
 #pragma unroll
@@ -1005,7 +1047,7 @@ void paged_prefill_kernel(PrefillParams p) {
     load_v(j0, 0);
     if constexpr (!kDirect) store_k(1);
     load_k(j0, 0);
-    sign_q();
+    if constexpr (kDirect) sign_q();
     find_pages(j0 + 1);
     if constexpr (kDirect) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -1020,12 +1062,19 @@ void paged_prefill_kernel(PrefillParams p) {
         find_pages(j + 2);
       }
       __syncthreads();
-      if (kDirect && j + 1 < j1) {
-        load_tile(j + 1, buf ^ 1);
+      if constexpr (kDirect) {
+        const auto loads = spread_load(j + 1, buf ^ 1, j + 1 < j1);
         find_pages(j + 2);
+        // (A wave without work in the step: apart from the step's condition, or the compiler
+        // joins the two and copies accumulators.)
+        int first = key0;
+        asm("" : "+s"(first));
+        if (first > any_to) static_unroll<NQ + 2 * ND>(loads);
+        step(key0, buf, 0, sa, sb, loads);
+      } else {
+        step(key0, buf, 0, sa, sb, nothing);
       }
-      step(key0, buf, 0, sa, sb);
-      step(key0 + 32, buf, 32, sb, sa);
+      step(key0 + 32, buf, 32, sb, sa, nothing);
     };
     if constexpr (kUnroll) {
       // Two tiles a round: the buffers are then constants, and part of the LDS reads' offsets.
