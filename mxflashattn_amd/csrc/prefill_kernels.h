@@ -1191,16 +1191,20 @@ void paged_prefill_kernel(PrefillParams p) {
 }
 
 // Joins the pieces of one row tile: workgroup (slot, kv head; part) where the slot holds a
-// tile's first piece, a thread for four dims of every kParts * kJoinRows-th row.
+// tile's first piece, a thread for four dims of kPer rows, in one pass with the running
+// reference and sum of each, kAhead pieces' loads at a time (16 heads on one kv head, some 200
+// tokens on up to 6k keys, 20 pieces a tile: 65.3 us with a piece's loads at a time, 45.6).
 constexpr int kPrefillJoinThreads = 256;
 constexpr int kPrefillJoinParts = 4;
 
 template <int HD, typename T>
 __global__ __launch_bounds__(kPrefillJoinThreads) void paged_prefill_join_kernel(PrefillParams p) {
   constexpr int kRows = kPrefillRows;
-  constexpr int kJoinRows = kPrefillJoinThreads / (HD / 4);
+  constexpr int kTogether = kPrefillJoinThreads / (HD / 4);  // rows
+  constexpr int kPer = kRows / kPrefillJoinParts / kTogether;
+  constexpr int kAhead = 16 / kPer;
   const int at = blockIdx.x;  // slot * hkv + kv head
-  const int slot = at / p.hkv, kvh = at - slot * p.hkv;
+  const int slot = div_by(at, p.hkv, p.hkv_mul), kvh = at - slot * p.hkv;
   if (slot >= *p.ws_total) return;
   const int4 d = p.ws_desc[at];
   const int pieces = d.x;
@@ -1208,33 +1212,60 @@ __global__ __launch_bounds__(kPrefillJoinThreads) void paged_prefill_join_kernel
   const PrefillSeq sq = prefill_seq(p, d.y);
   const int chunk = threadIdx.x % (HD / 4);
   const int rows = min(kRows, sq.n * p.gq - d.z * kRows);
-  for (int r = blockIdx.y * kJoinRows + threadIdx.x / (HD / 4); r < rows;
-       r += kPrefillJoinParts * kJoinRows) {
-    const int row = d.z * kRows + r;
-    const int tok = row / p.gq, head = kvh * p.gq + row % p.gq;
-    float m = -INFINITY;
-    for (int i = 0; i < pieces; ++i)
-      m = fmaxf(m, p.ws_lse[(at + (int64_t)i * p.hkv) * kRows + r]);
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < pieces; ++i) {
-      const int64_t a = (at + (int64_t)i * p.hkv) * kRows + r;
-      const float lse = p.ws_lse[a];
-      const float w = lse == -INFINITY ? 0.f : fast_exp2(lse - m);
-      const float4 x = *reinterpret_cast<const float4 *>(p.ws_o + a * HD + 4 * chunk);
-      sum += w;
-      acc.x += w * x.x;
-      acc.y += w * x.y;
-      acc.z += w * x.z;
-      acc.w += w * x.w;
+  if ((int)blockIdx.y * (kTogether * kPer) >= rows) return;
+  const int r0 = blockIdx.y * (kTogether * kPer) + threadIdx.x / (HD / 4);
+  float m[kPer], sum[kPer];
+  float4 acc[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    m[u] = -INFINITY;
+    sum[u] = 0.f;
+    acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int i = 0; i < pieces; i += kAhead) {
+    float lse[kAhead][kPer];
+    float4 x[kAhead][kPer];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int64_t first = (at + (int64_t)min(i + a, pieces - 1) * p.hkv) * kRows;
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        const int64_t r = first + min(r0 + u * kTogether, rows - 1);
+        lse[a][u] = p.ws_lse[r];
+        x[a][u] = *reinterpret_cast<const float4 *>(p.ws_o + r * HD + 4 * chunk);
+      }
     }
-    float den = sum;
-    if (p.sinks) den += fast_exp2(p.sinks[head] * kPrefillLog2e - m);
-    const float inv = sum == 0.f ? 0.f : 1.f / den;
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      if (i + a >= pieces) break;
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        const float top = fmaxf(m[u], lse[a][u]);
+        // No key seen so far, or none in the piece: weight 0. (A NaN stays one.)
+        const float f = m[u] == -INFINITY ? 0.f : fast_exp2(m[u] - top);
+        const float w = lse[a][u] == -INFINITY ? 0.f : fast_exp2(lse[a][u] - top);
+        m[u] = top;
+        sum[u] = sum[u] * f + w;
+        acc[u].x = acc[u].x * f + w * x[a][u].x;
+        acc[u].y = acc[u].y * f + w * x[a][u].y;
+        acc[u].z = acc[u].z * f + w * x[a][u].z;
+        acc[u].w = acc[u].w * f + w * x[a][u].w;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int r = r0 + u * kTogether;
+    if (r >= rows) continue;
+    const int row = d.z * kRows + r;
+    const int tok = div_by(row, p.gq, p.gq_mul), head = kvh * p.gq + row - tok * p.gq;
+    float den = sum[u];
+    if (p.sinks) den += fast_exp2(p.sinks[head] * kPrefillLog2e - m[u]);
+    const float inv = sum[u] == 0.f ? 0.f : 1.f / den;
     *reinterpret_cast<uint2 *>(p.out + (int64_t)(sq.start + tok) * p.o_st +
                                (int64_t)head * p.o_sh + 8 * chunk) =
-        make_uint2(Prod32<T>::pack(acc.x * inv, acc.y * inv),
-                   Prod32<T>::pack(acc.z * inv, acc.w * inv));
+        make_uint2(Prod32<T>::pack(acc[u].x * inv, acc[u].y * inv),
+                   Prod32<T>::pack(acc[u].z * inv, acc[u].w * inv));
   }
 }
 
