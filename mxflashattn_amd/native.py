@@ -182,6 +182,10 @@ _PACKAGE_SIGNATURES = {
          _i64, _i64, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
 }
 
+# Entry points that launch a pair of kernels over one workspace: called with the interpreter
+# lock held, so that no other thread's call of one of them on the same stream comes between.
+_HELD = ("mxfa_package_decode_rows_launch", "mxfa_package_prefill_launch")
+
 _load_lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 _load_error: str | None = None
@@ -203,13 +207,15 @@ def library() -> ctypes.CDLL:
             raise NativeLibraryError(_load_error)
         try:
             lib = ctypes.CDLL(str(LIB_PATH))
+            held = ctypes.PyDLL(str(LIB_PATH))
         except OSError as exc:
             _load_error = f"native library failed to load: {exc}"
             raise NativeLibraryError(_load_error) from exc
         for name, (restype, argtypes) in (*_SIGNATURES.items(), *_PACKAGE_SIGNATURES.items()):
-            fn = getattr(lib, name)
+            fn = getattr(held if name in _HELD else lib, name)
             fn.restype = restype
             fn.argtypes = argtypes
+            setattr(lib, name, fn)
         version = lib.mxfa_abi_version()
         if version != ABI_VERSION:
             _load_error = f"native library ABI {version} does not match {ABI_VERSION}"
@@ -338,19 +344,24 @@ class _Workspace:
 WORKSPACE = _Workspace()
 
 
+# Of the calls in _HELD, apart from the other calls' (which release the interpreter lock).
+_HELD_WORKSPACE = _Workspace()
+
+
 def _own_workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Workspace of a call whose captures may be replayed beside each other: a graph gets
     memory of its own pool instead of the stream's buffer."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return WORKSPACE.get(device, stream, nbytes)
+    return _HELD_WORKSPACE.get(device, stream, nbytes)
 
 
 def retired_workspace_bytes() -> int:
     """Bytes of workspaces replaced by larger ones and kept alive, over the
     ctypes path's cache and the torch operator's."""
     op = torch_op()
-    return WORKSPACE.retired_bytes() + (op.workspace_bytes()[1] if op is not None else 0)
+    retired = WORKSPACE.retired_bytes() + _HELD_WORKSPACE.retired_bytes()
+    return retired + (op.workspace_bytes()[1] if op is not None else 0)
 
 
 def _poison(out: torch.Tensor | None, ws: torch.Tensor | None = None) -> None:

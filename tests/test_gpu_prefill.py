@@ -290,6 +290,42 @@ def test_streams_do_not_share_a_workspace(device):
 
 
 @pytest.mark.parametrize("torch_op", [True, False], ids=["op", "ctypes"])
+def test_threads_on_one_stream(device, monkeypatch, torch_op):
+    """Calls of several threads on one stream: each pair of launches stays together."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    monkeypatch.setattr(native, "USE_TORCH_OP", torch_op)
+    stream = torch.cuda.Stream()
+    calls = []
+    for seed in range(4):
+        codes = INT8 if seed % 2 else None
+        p = make_paged([6000, 3000], 2, 128, BF16, 16, codes=codes, seed=seed).to(device)
+        q, cu = packed_q([8, 20], 8, 128, BF16, seed)
+        calls.append((q.to(device), p, cu.to(device)))
+
+    def run(i):
+        q, p, cu = calls[i]
+        if i == 3:  # the decode of the same rows
+            return mx.paged_decode_split(q[:2], p.kc, p.vc, p.table, p.lens, 0.1, num_splits=64,
+                                         k_scale=p.ks, v_scale=p.vs)
+        return mx.paged_prefill(q, p.kc, p.vc, cu, p.table, p.lens, 0.1, k_scale=p.ks,
+                                v_scale=p.vs)
+
+    def many(i):
+        with torch.cuda.stream(stream):
+            return [run(i) for _ in range(25)]
+
+    with torch.cuda.stream(stream):
+        want = [run(i) for i in range(4)]
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(4) as pool:
+        got = list(pool.map(many, range(4)))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
+
+
+@pytest.mark.parametrize("torch_op", [True, False], ids=["op", "ctypes"])
 def test_captured_calls_side_by_side(device, monkeypatch, torch_op):
     """Two graphs captured on one stream, replayed on two at once beside eager calls on the
     first: cut tiles' pieces of the one never meet the other's."""
