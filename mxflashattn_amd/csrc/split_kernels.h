@@ -814,9 +814,11 @@ __device__ __forceinline__ uint32_t run_range(const DecodeParams &p, const int32
   constexpr int VB = kF8 ? VD : 2 * VD;      // V bytes per lane and token
   constexpr int U = 4;                       // V tokens per lane (token 4r+u in DPP row r)
   constexpr bool kRows = kF8 >= kRowsE4m3;   // 8-bit rows with a scale each
-  // PV's element type. A row's scale times a weight may lie below fp16's range:
-  // an fp16 call on such rows holds V as bf16 and P as the sum of two bf16.
-  constexpr bool kSplitP = kRows && std::is_same_v<T, F16>;
+  // PV on such rows: V as bf16 and P as the sum of two bf16 (16 bits of precision).
+  // A row's scale times a weight may lie below fp16's range, and one bf16 of it is
+  // off by 2^-9 with nothing in the denominator (the weights without the scale) that
+  // goes along: twice the plain form's error where few keys make up a row.
+  constexpr bool kSplitP = kRows;
   using TV = std::conditional_t<kSplitP, BF16, T>;
   constexpr int NPG = kLanePages ? 1 + U : 1;
   // 8-byte V slots (128-byte rows): lanes c and c^8 of a row load 16 bytes
@@ -1914,11 +1916,11 @@ static int launch_partial_s(const DecodeParams &p, const Grid &g, hipStream_t st
         return hipGetLastError() == hipSuccess ? MXFA_OK : MXFA_ELAUNCH;
       }
     }
-    // Rows with a scale each: a set holds their scales too, and with options or
-    // fp16's split weights a third set of 128-byte rows does not fit two waves per
-    // SIMD.
+    // Rows with a scale each: a set holds their scales too, and with options, more
+    // than four columns or fp16's products a third set of 128-byte rows does not fit
+    // two waves per SIMD.
     constexpr int kSets = kF8 >= kRowsE4m3 && kRowBytes<HD, kF8> == 128 &&
-                                  (kExtras || std::is_same_v<T, F16>)
+                                  (kExtras || HR > 1 || std::is_same_v<T, F16>)
                               ? 2
                               : kNbuf<HD, kF8>;
     hipLaunchKernelGGL((split_partial_kernel<HD, HR, T, kF8, false, kSets, WAVES, kExtras,
